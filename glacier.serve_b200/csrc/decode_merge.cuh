@@ -16,7 +16,8 @@ namespace gkv {
 
 // The work list a launch runs: `w` itself, or (static step layout, w.dyn set) the pointers
 // and counts of the header the step's upload wrote at w.dyn.  The buffer comes from a host
-// copy ordered before the launch, so it may be read before pdl_wait.
+// copy, or a kernel (step_build.cu) that an ordinary launch has separated from this one, so it
+// may be read before pdl_wait.
 __device__ __forceinline__ DecodeWork resolve_work(DecodeWork w) {
     if (!w.dyn) return w;
     const int32_t* h = reinterpret_cast<const int32_t*>(w.dyn);
@@ -26,7 +27,8 @@ __device__ __forceinline__ DecodeWork resolve_work(DecodeWork w) {
     w.n_merge = __ldg(h + kHdrMerge);
     w.n_deferred = __ldg(h + kHdrDeferred);
     w.n_deferred_long = __ldg(h + kHdrDeferredLong);
-    w.tables = at(kHdrTables);
+    const unsigned long long own_tables = __ldg(reinterpret_cast<const unsigned long long*>(h + kHdrTablesPtr));
+    w.tables = own_tables ? reinterpret_cast<const int32_t*>(own_tables) : at(kHdrTables);
     w.ctx_lens = at(kHdrCtx);
     w.piece_seg = at(kHdrPseg);
     w.piece_c0 = at(kHdrPc0);

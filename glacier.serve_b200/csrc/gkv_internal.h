@@ -164,6 +164,7 @@ struct StepWorkspace {
     DecodeWork work{};
     const int64_t* d_slots = nullptr;
     bool uploaded = false;
+    bool built = false;          // the step came from gkv_step_build and no launch has followed it
     std::vector<int32_t> h_ctx;  // ctx_lens of the uploaded step
     WorkList wl;                 // the uploaded step's work list (kept for its capacity)
     // chunked prefill: pinned + device buffer of its work items / work list, and q in the
@@ -245,6 +246,7 @@ int step_append(Pool* p, int32_t layer, const float* d_k, const float* d_v, int3
 int step_decode_lse(Pool* p, int32_t layer, const float* d_q, float* d_out, float* d_lse,
                     int32_t n_heads, float scale, const float* d_sinks, cudaStream_t st);
 int step_set_static(Pool* p, bool enable);
+int step_build(Pool* p, const gkv_step_io* io, int32_t batch, cudaStream_t st);
 int step_reserve(Pool* p, int32_t max_batch, int32_t max_blocks, int32_t max_tokens,
                  int32_t n_heads);
 int step_prefill(Pool* p, int32_t layer, const void* d_q, int32_t q_dtype, float* d_out,
@@ -253,6 +255,10 @@ int step_prefill(Pool* p, int32_t layer, const void* d_q, int32_t q_dtype, float
 int step_rope_append(Pool* p, int32_t layer, float* d_q, const float* d_k, const float* d_v, int32_t n_tok,
                      int32_t n_heads, const int32_t* positions, const gkv_rope_desc* rope,
                      const gkv_qkv_prologue* pro, cudaStream_t st);
+int step_mrope_append(Pool* p, int32_t layer, const gkv_qkv_io* io, int32_t n_tok, int32_t n_heads,
+                      const int32_t* d_positions, int64_t pos_stride, const gkv_mrope_desc* rope,
+                      const gkv_qkv_prologue* pro, cudaStream_t st);
+int step_prompt(Pool* p, const gkv_prompt_desc* r, cudaStream_t st);
 void rope_inv_freq(float freq_base, int32_t rope_dim, const float* factors, float* out);
 void step_free(Pool* p);
 

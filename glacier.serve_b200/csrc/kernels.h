@@ -47,10 +47,37 @@ struct ArenaGeom {
 enum : int {
     kHdrTok, kHdrBatch, kHdrMaxBlocks, kHdrSlots, kHdrMerge, kHdrDeferred, kHdrDeferredLong, kHdrWorkers,
     kHdrTables, kHdrCtx, kHdrPseg, kHdrPc0, kHdrPc1, kHdrPslot, kHdrPmerge, kHdrWbeg, kHdrMseg, kHdrMs0,
-    kHdrMns, kHdrMdef, kHdrInts
+    kHdrMns, kHdrMdef, kHdrOffsetsEnd,
+    // 64-bit address of the block tables when they are the caller's own (a step built on the
+    // device); 0: the tables are in the buffer, at kHdrTables
+    kHdrTablesPtr = kHdrOffsetsEnd, kHdrInts = kHdrTablesPtr + 2
 };
+static_assert(kHdrTablesPtr % 2 == 0, "the table address is read as one 64-bit word");
 constexpr size_t kHdrBytes = 128;  // the slot mapping starts here
 static_assert(kHdrInts * 4 <= static_cast<int>(kHdrBytes), "step header");
+
+// ---- step metadata built on the device (step_build.cu) ----
+constexpr int kMaxBuildBatch = 4096;  // requests of one built step
+struct StepBuildArgs {
+    // the caller's arrays (device): see gkv_step_io
+    const int32_t *ctx_lens, *new_lens, *new_blocks;
+    int32_t* tables;
+    int32_t *ctx_out, *cu_new, *positions, *counts;  // each may be nullptr
+    int64_t* slots;                                  // may be nullptr
+    int64_t table_stride;
+    int32_t n_new_blocks, max_tokens, batch;
+    // the pool
+    int32_t block_size, total_blocks, heads_kv, n_workers;
+    // the packed step buffer, with every array at the offset of the reservation's maxima
+    unsigned char* meta;
+    int32_t off_ctx, off_pseg, off_pc0, off_pc1, off_pslot, off_pmerge, off_wbeg, off_mseg, off_ms0, off_mns, off_mdef;
+    int32_t* scratch;                                // 2 * batch * heads_kv ints
+    int* err;
+};
+cudaError_t launch_step_build(const StepBuildArgs& a, cudaStream_t st);
+// An empty kernel, launched without programmatic overlap: what follows it on the stream sees
+// everything before it, even where it reads before its own pdl_wait.
+cudaError_t launch_order(cudaStream_t st);
 
 // ---- kv append ----
 // Writes token i's K/V rows into slot slots[i] (or `single_slot` when slots == nullptr and
@@ -81,6 +108,44 @@ struct RopeAppendParams {
 // head_dim in {32, 64, 128, 256}, rope_dim even, <= head_dim, (rope_dim/2) % (head_dim/32) == 0.
 bool rope_append_supported(const ArenaGeom& g, int rope_dim);
 cudaError_t launch_rope_append(const ArenaGeom& g, const RopeAppendParams& p, cudaStream_t st);
+
+// ---- rotary positions with several axes + q/k/v prologue + KV append (mrope_append.cu) ----
+constexpr int kMropeMaxPairs = 128;
+struct MropeParams {
+    int layer;
+    const void *q, *k, *v;               // [n_tok][heads][dim] with strides, of type in_dtype
+    void *q_out, *k_out, *v_out;         // dense, of type out_dtype; k_out / v_out may be nullptr
+    int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;
+    int in_dtype, out_dtype;
+    int n_tok, n_heads;
+    const int32_t* dyn_tok;              // static step layout: the row count, read on the device
+    const int32_t* positions;            // device [axis][n_tok], pos_stride apart
+    int64_t pos_stride;
+    int rope_dim, style;
+    float mscale;
+    const float *q_bias, *k_bias, *v_bias, *q_norm, *k_norm;  // device or nullptr
+    float eps;
+    const int64_t* slots;                // device [n_tok]
+    int* err;
+    float inv_freq[kMropeMaxPairs];
+    uint8_t axis[kMropeMaxPairs];
+};
+// head_dim in {32, 64, 128, 256}, v_head_dim a multiple of 8, every head row 16-byte aligned.
+cudaError_t launch_mrope_append(const ArenaGeom& g, const MropeParams& p, cudaStream_t st);
+
+// ---- causal attention of packed prompts (prompt_attention*.cu) ----
+struct PromptArgs {
+    const void *q, *k, *v;               // [total][heads][dim] with strides (elements)
+    void* out;                           // dense [total][n_heads][dv]
+    float* lse;                          // [total][n_heads] or nullptr
+    const float* sinks;                  // [n_heads] or nullptr
+    const int32_t* cu;                   // [batch + 1]
+    int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;
+    int batch, total, n_heads, heads_kv, d, dv, dtype;
+    float scale;
+    int* err;
+};
+cudaError_t launch_prompt_simt(const PromptArgs& a, cudaStream_t st);
 
 // ---- block copy ----
 // ops: [n][3] int32 (src, dst, valid_tokens) in device memory.

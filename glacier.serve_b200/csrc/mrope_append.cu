@@ -1,0 +1,234 @@
+// Rotary positions with several axes, fused with the q/k/v prologue and the KV append.
+//
+// gkv_rope_append's steps (bias, per-head RMSNorm of q and k, rotation, Store) for tokens whose
+// position has several axes, as image and video patches have: pair i of a head turns by
+//   angle_i = position[axis(i)] * inv_freq[i],   (a, b) -> (a cos - b sin, b cos + a sin) * mscale.
+// The angle is the exact product in 64 bits (31 + 24 bits of factors), reduced by pi/2 there and only
+// then rounded: at position 10^6 a product in 32 bits is off by up to 2^-5 rad.  Everything else is
+// 32 bits, rounded once to each destination's type.
+//
+// Roofline: HBM for prompts, launch latency for single tokens.  A block takes a few tokens (one
+// where there are few), puts their cos and sin into shared memory once for all heads, and hands
+// each group of head_dim / 16 lanes one head row: a lane holds 8 pairs, read as two vectors of 8
+// elements (pairs (i, i + R/2)) or one of 16 (pairs (2i, 2i + 1)), so partners meet in a lane and
+// the norm's sum crosses lanes only log2(head_dim / 16) times.
+#include "gkv_device.cuh"
+#include "kernels.h"
+#include "rope_math.cuh"
+#include "../../include/glacier_kv.h"
+
+namespace gkv {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxTokens = 4;  // tokens per block
+
+__device__ __forceinline__ float2 unpack(uint32_t w, __nv_bfloat16) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ float2 unpack(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+
+// 8 consecutive elements as floats, from a 16-byte boundary.  Plain loads, not the read-only path:
+// q may be rewritten in place by the lane that read it.
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+    const uint4 w = *reinterpret_cast<const uint4*>(p);
+    const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float2 f = unpack(q[e], T{});
+        x[2 * e] = f.x;
+        x[2 * e + 1] = f.y;
+    }
+}
+
+// 8 consecutive elements, rounded to nearest even (fp8: times `inv`, the reciprocal of the head's
+// scale, saturated).
+__device__ __forceinline__ void store8(float* p, const float (&x)[8], float) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&x)[8], float) {
+    *reinterpret_cast<uint4*>(p) =
+        make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+}
+__device__ __forceinline__ void store8(__half* p, const float (&x)[8], float) {
+    *reinterpret_cast<uint4*>(p) =
+        make_uint4(pack_f16x2(x[0], x[1]), pack_f16x2(x[2], x[3]), pack_f16x2(x[4], x[5]), pack_f16x2(x[6], x[7]));
+}
+__device__ __forceinline__ void store8(__nv_fp8_e4m3* p, const float (&x)[8], float inv) {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        w[e] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * e] * inv, x[2 * e + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+    *reinterpret_cast<uint2*>(p) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+}
+__device__ __forceinline__ void store8_as(void* base, int dtype, int64_t at, const float (&x)[8]) {
+    if (dtype == GKV_DTYPE_F32) store8(static_cast<float*>(base) + at, x, 1.f);
+    else if (dtype == GKV_DTYPE_BF16) store8(static_cast<__nv_bfloat16*>(base) + at, x, 1.f);
+    else store8(static_cast<__half*>(base) + at, x, 1.f);
+}
+
+// x += bias, element by element (biases need no alignment).
+__device__ __forceinline__ void add8(const float* bias, float (&x)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] += __ldg(bias + e);
+}
+
+// T: the type of q, k and v; KV: the arena's.
+template <typename T, typename KV>
+__global__ void __launch_bounds__(kThreads) mrope_append_kernel(const ArenaGeom g, const __grid_constant__ MropeParams a, const int tokens) {
+    pdl_launch_dependents();  // the decode that follows waits for this grid before reading q or the arena
+    __shared__ float2 turn[kMaxTokens * kMropeMaxPairs];  // (cos, sin) * mscale of each token's pairs
+    __shared__ int64_t slot_of[kMaxTokens];
+    const int n_tok = a.dyn_tok ? min(__ldg(a.dyn_tok), a.n_tok) : a.n_tok;
+    const int t0 = blockIdx.x * tokens;
+    const int nt = min(tokens, n_tok - t0);
+    if (nt <= 0) return;
+    const int half = a.rope_dim / 2;
+    for (int i = threadIdx.x; i < nt * half; i += kThreads) {
+        const int t = i / half, j = i - t * half;
+        const int pos = __ldg(a.positions + a.axis[j] * a.pos_stride + t0 + t);
+        float s, c;
+        rope_sincos_f64(static_cast<double>(pos) * static_cast<double>(a.inv_freq[j]), s, c);
+        turn[i] = make_float2(c * a.mscale, s * a.mscale);
+    }
+    if (threadIdx.x < nt) {
+        int64_t s = __ldg(a.slots + t0 + threadIdx.x);
+        if (s >= static_cast<int64_t>(g.total_blocks) * g.block_size) {
+            atomicOr(a.err, kErrBadSlot);
+            s = -1;
+        }
+        slot_of[threadIdx.x] = s;
+    }
+    __syncthreads();
+
+    const int d = g.head_dim, hk = g.heads_kv, lane = threadIdx.x & 31;
+    const int tpr = d / 16;  // lanes of a head row: 2, 4, 8 or 16
+    const int rows = a.n_heads + hk;
+    const int units = nt * rows * tpr;
+    const bool neox = a.style == GKV_ROPE_NEOX;
+    // whole warps run every pass: the norm's sums cross lanes
+    for (int i = threadIdx.x; i - lane < units; i += kThreads) {
+        const bool live = i < units;
+        const int row = live ? i / tpr : 0, u = live ? (i - row * tpr) * 8 : 0;  // pairs u .. u + 7 of d / 2
+        const int t = row / rows, r = row - t * rows;
+        const bool is_q = r < a.n_heads;
+        const int h = is_q ? r : r - a.n_heads;
+        const int64_t tok = t0 + t;
+        // NEOX: 8 first elements of pairs, then their 8 partners; the unrotated elements [R, d) pair
+        // up as halves too.  Interleaved: 16 adjacent elements.  R is a multiple of 16, so a vector
+        // lies on one side of it.
+        const int ia = neox ? (u < half ? u : u + half) : 2 * u;
+        const int ib = neox ? (u < half ? u + half : u + d / 2) : 2 * u + 8;
+        const T* src = is_q ? static_cast<const T*>(a.q) + tok * a.q_ts + h * a.q_hs : static_cast<const T*>(a.k) + tok * a.k_ts + h * a.k_hs;
+        float x[8], y[8];
+        load8(src + ia, x);
+        load8(src + ib, y);
+        const float* bias = is_q ? a.q_bias : a.k_bias;
+        if (bias) {
+            add8(bias + h * d + ia, x);
+            add8(bias + h * d + ib, y);
+        }
+        if (a.q_norm || a.k_norm) {  // the same for the whole grid; a row without a weight ignores the sum
+            float p = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p = fmaf(x[e], x[e], fmaf(y[e], y[e], p));
+            for (int o = tpr >> 1; o >= 1; o >>= 1) p += __shfl_xor_sync(~0u, p, o);
+            if (const float* w = is_q ? a.q_norm : a.k_norm) {
+                const float inv = 1.f / sqrtf(p / static_cast<float>(d) + a.eps);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] *= inv * __ldg(w + ia + e);
+                    y[e] *= inv * __ldg(w + ib + e);
+                }
+            }
+        }
+        if (!live) continue;
+        if (u < half) {  // all 8 pairs, or none
+            const float2* w = turn + t * half + u;
+            if (neox) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float p = x[e];
+                    x[e] = p * w[e].x - y[e] * w[e].y;
+                    y[e] = y[e] * w[e].x + p * w[e].y;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const float2 w0 = w[e / 2], w1 = w[4 + e / 2];
+                    const float p = x[e], q = y[e];
+                    x[e] = p * w0.x - x[e + 1] * w0.y;
+                    x[e + 1] = x[e + 1] * w0.x + p * w0.y;
+                    y[e] = q * w1.x - y[e + 1] * w1.y;
+                    y[e + 1] = y[e + 1] * w1.x + q * w1.y;
+                }
+            }
+        }
+        if (void* out = is_q ? a.q_out : a.k_out) {
+            const int64_t at = (tok * (is_q ? a.n_heads : hk) + h) * d;
+            store8_as(out, a.out_dtype, at + ia, x);
+            store8_as(out, a.out_dtype, at + ib, y);
+        }
+        const int64_t slot = slot_of[t];
+        if (!is_q && slot >= 0) {
+            const int64_t blk = slot / g.block_size;
+            KV* dst = static_cast<KV*>(g.k) + blk * g.k_block_stride + a.layer * g.k_layer_stride + h * g.k_head_stride +
+                      (slot - blk * g.block_size) * d;
+            const float inv = g.k_inv ? __ldg(g.k_inv + a.layer * hk + h) : 1.f;
+            store8(dst + ia, x, inv);
+            store8(dst + ib, y, inv);
+        }
+    }
+    // v: 8 elements per lane
+    const int dv = g.v_head_dim, vpr = dv / 8;
+    for (int i = threadIdx.x; i < nt * hk * vpr; i += kThreads) {
+        const int row = i / vpr, e = (i - row * vpr) * 8;
+        const int t = row / hk, h = row - t * hk;
+        const int64_t tok = t0 + t;
+        float x[8];
+        load8(static_cast<const T*>(a.v) + tok * a.v_ts + h * a.v_hs + e, x);
+        if (a.v_bias) add8(a.v_bias + h * dv + e, x);
+        if (a.v_out) store8_as(a.v_out, a.out_dtype, (tok * hk + h) * dv + e, x);
+        const int64_t slot = slot_of[t];
+        if (slot < 0) continue;
+        const int64_t blk = slot / g.block_size;
+        KV* dst = static_cast<KV*>(g.v) + blk * g.v_block_stride + a.layer * g.v_layer_stride + h * g.v_head_stride +
+                  (slot - blk * g.block_size) * dv + e;
+        store8(dst, x, g.v_inv ? __ldg(g.v_inv + a.layer * hk + h) : 1.f);
+    }
+}
+
+template <typename T, typename KV>
+cudaError_t launch_typed(const ArenaGeom& g, const MropeParams& p, cudaStream_t st) {
+    // one token per block until the card is full
+    const int tokens = p.n_tok <= 148 * 8 ? 1 : kMaxTokens;
+    const int64_t blocks = (static_cast<int64_t>(p.n_tok) + tokens - 1) / tokens;
+    mrope_append_kernel<T, KV><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(g, p, tokens);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_arena(const ArenaGeom& g, const MropeParams& p, cudaStream_t st) {
+    if (g.dtype == GKV_DTYPE_BF16) return launch_typed<T, __nv_bfloat16>(g, p, st);
+    if (g.dtype == GKV_DTYPE_F16) return launch_typed<T, __half>(g, p, st);
+    if (g.dtype == GKV_DTYPE_FP8_E4M3) return launch_typed<T, __nv_fp8_e4m3>(g, p, st);
+    return launch_typed<T, float>(g, p, st);
+}
+
+}  // namespace
+
+cudaError_t launch_mrope_append(const ArenaGeom& g, const MropeParams& p, cudaStream_t st) {
+    if (p.n_tok <= 0) return cudaSuccess;
+    if (p.in_dtype == GKV_DTYPE_BF16) return launch_arena<__nv_bfloat16>(g, p, st);
+    if (p.in_dtype == GKV_DTYPE_F16) return launch_arena<__half>(g, p, st);
+    return launch_arena<float>(g, p, st);
+}
+
+}  // namespace gkv

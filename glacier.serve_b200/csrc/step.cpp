@@ -352,6 +352,7 @@ int step_set_static(Pool* p, bool enable) {
     }
     ws.static_mode = enable;
     ws.uploaded = false;  // the next upload writes the layout the launches will read
+    ws.built = false;
     return GKV_OK;
 }
 
@@ -489,7 +490,8 @@ int step_upload(Pool* p, const int32_t* tables, int32_t batch, int32_t max_block
         hd[kHdrWorkers] = static_cast<int32_t>(n_workers);
         const size_t offs[] = {L.tables, L.ctx, L.pseg, L.pc0, L.pc1, L.pslot, L.pmerge,
                                L.wbeg, L.mseg, L.ms0, L.mns, L.mdef};
-        for (int k = 0; k < kHdrInts - kHdrTables; ++k) hd[kHdrTables + k] = static_cast<int32_t>(offs[k]);
+        for (int k = 0; k < kHdrOffsetsEnd - kHdrTables; ++k) hd[kHdrTables + k] = static_cast<int32_t>(offs[k]);
+        hd[kHdrTablesPtr] = hd[kHdrTablesPtr + 1] = 0;
         memcpy(h + L.hdr, hd, sizeof(hd));
     }
     cudaError_t e = cudaSuccess;
@@ -550,6 +552,85 @@ int step_upload(Pool* p, const int32_t* tables, int32_t batch, int32_t max_block
     ws.n_tok = n_tok;
     ws.up_max_blocks = max_blocks;
     ws.uploaded = true;
+    ws.built = false;
+    return GKV_OK;
+}
+
+int step_build(Pool* p, const gkv_step_io* io, int32_t batch, cudaStream_t st) {
+    StepWorkspace& ws = p->ws;
+    if (!io) return set_error(GKV_EINVAL, "step arrays are NULL");
+    if (!ws.static_mode)
+        return set_error(GKV_ESTATE, "a step is built on the device in the static step layout only (gkv_step_set_static)");
+    if (batch < 0 || batch > ws.max_batch || batch > kMaxBuildBatch)
+        return set_error(GKV_EINVAL, "batch %d outside [0, %d]", batch, std::min(ws.max_batch, kMaxBuildBatch));
+    if (io->max_tokens < 0 || io->max_tokens > ws.max_tokens)
+        return set_error(GKV_EINVAL, "max_tokens %d outside the static step reservation [0, %d]", io->max_tokens, ws.max_tokens);
+    if (io->n_new_blocks < 0) return set_error(GKV_EINVAL, "negative n_new_blocks %d", io->n_new_blocks);
+    if (batch > 0 && (!io->d_ctx_lens || !io->d_new_lens || !io->d_block_tables))
+        return set_error(GKV_EINVAL, "ctx_lens/new_lens/block_tables is NULL");
+    if (io->n_new_blocks > 0 && !io->d_new_blocks) return set_error(GKV_EINVAL, "new_blocks is NULL");
+    if (batch > 0 && io->table_stride < 1) return set_error(GKV_EINVAL, "table_stride %d < 1", io->table_stride);
+    if (batch > 0 && (io->d_ctx_out == io->d_ctx_lens || io->d_ctx_out == io->d_new_lens))
+        return set_error(GKV_EINVAL, "ctx_out must not be ctx_lens or new_lens (every block of the kernel reads those)");
+    const int64_t workers = static_cast<int64_t>(ws.n_ctas_max) * ws.cfg.warps;
+    const int64_t n_seg = static_cast<int64_t>(ws.max_batch) * p->desc.heads_kv;
+    const MetaLayout L = meta_layout(ws.max_tokens, ws.max_batch, 0, workers + n_seg, workers, n_seg);
+    if (L.total > ws.meta_cap || static_cast<size_t>(n_seg) * 8 > ws.meta_cap || L.total > 0x7fffffff)
+        return set_error(GKV_ESTATE, "static step buffer too small");
+    StepBuildArgs a{};
+    a.ctx_lens = io->d_ctx_lens;
+    a.new_lens = io->d_new_lens;
+    a.new_blocks = io->d_new_blocks;
+    a.tables = io->d_block_tables;
+    a.ctx_out = io->d_ctx_out;
+    a.cu_new = io->d_cu_new;
+    a.positions = io->d_positions;
+    a.counts = io->d_counts;
+    a.slots = io->d_slots;
+    a.table_stride = io->table_stride;
+    a.n_new_blocks = io->n_new_blocks;
+    a.max_tokens = io->max_tokens;
+    a.batch = batch;
+    a.block_size = p->desc.block_size;
+    a.total_blocks = p->desc.total_blocks;
+    a.heads_kv = p->desc.heads_kv;
+    a.n_workers = static_cast<int32_t>(workers);
+    a.meta = reinterpret_cast<unsigned char*>(ws.d_meta[0]);
+    a.off_ctx = static_cast<int32_t>(L.ctx);
+    a.off_pseg = static_cast<int32_t>(L.pseg);
+    a.off_pc0 = static_cast<int32_t>(L.pc0);
+    a.off_pc1 = static_cast<int32_t>(L.pc1);
+    a.off_pslot = static_cast<int32_t>(L.pslot);
+    a.off_pmerge = static_cast<int32_t>(L.pmerge);
+    a.off_wbeg = static_cast<int32_t>(L.wbeg);
+    a.off_mseg = static_cast<int32_t>(L.mseg);
+    a.off_ms0 = static_cast<int32_t>(L.ms0);
+    a.off_mns = static_cast<int32_t>(L.mns);
+    a.off_mdef = static_cast<int32_t>(L.mdef);
+    // the second metadata buffer is idle in the static layout
+    a.scratch = reinterpret_cast<int32_t*>(ws.d_meta[1]);
+    a.err = ws.d_err;
+    cudaError_t e = launch_step_build(a, st);
+    if (e != cudaSuccess) return cuda_fail(e, "step_build launch");
+    p->last_launches += 1;
+    // what the launches of the step take from the host: fixed addresses, the reservation's grids
+    char* d = ws.d_meta[0];
+    DecodeWork& w = ws.work;
+    w = DecodeWork{};
+    w.tables = io->d_block_tables;
+    w.ctx_lens = reinterpret_cast<const int32_t*>(d + L.ctx);
+    w.max_blocks = io->table_stride;
+    w.n_ctas = ws.n_ctas_max;
+    w.merge_count = ws.d_merge_count;
+    w.dyn = reinterpret_cast<const unsigned char*>(d);
+    w.merge_grid = ws.static_merge_grid;
+    ws.d_slots = reinterpret_cast<const int64_t*>(d + L.slots);
+    ws.h_ctx.clear();
+    ws.batch = batch;
+    ws.n_tok = io->max_tokens;
+    ws.up_max_blocks = io->table_stride;
+    ws.uploaded = true;
+    ws.built = true;
     return GKV_OK;
 }
 
@@ -590,6 +671,7 @@ int step_append(Pool* p, int32_t layer, const float* d_k, const float* d_v, int3
                                      static_cast<int64_t>(p->desc.heads_kv) * p->desc.v_head_dim,
                                      ws.d_slots, 0, ws.static_mode ? ws.max_tokens : n_tok, ws.d_err, st, dyn_tok);
     if (e != cudaSuccess) return cuda_fail(e, "kv_append launch");
+    ws.built = false;
     p->last_launches += 1;
     return GKV_OK;
 }
@@ -643,6 +725,14 @@ static int decode_common(Pool* p, int32_t layer, const float* d_q, float* d_out,
     a.err = ws.d_err;
     a.lse = d_lse;
     int launches = 0;
+    if (ws.built) {
+        // the decode reads the step header before its pdl_wait: with nothing launched since the
+        // kernel that builds the header, an ordinary launch has to come between
+        cudaError_t e = launch_order(st);
+        if (e != cudaSuccess) return cuda_fail(e, "step order launch");
+        ws.built = false;
+        ++p->last_launches;
+    }
     cudaError_t e = launch_paged_decode(p->geom, ws.work, a, &launches, st);
     if (e != cudaSuccess) return cuda_fail(e, "paged_decode launch");
     p->last_launches += launches;
@@ -997,6 +1087,177 @@ int step_rope_append(Pool* p, int32_t layer, float* d_q, const float* d_k, const
     a.err = ws.d_err;
     cudaError_t e = launch_rope_append(p->geom, a, st);
     if (e != cudaSuccess) return cuda_fail(e, "rope_append launch");
+    ws.built = false;
+    p->last_launches += 1;
+    return GKV_OK;
+}
+
+namespace {
+
+// Whether a [rows][heads][dim] operand of `bytes`-byte elements keeps every head row on a 16-byte
+// boundary (strides in elements; a stride that is never taken does not count).
+bool rows_aligned(const void* p, int64_t tok_stride, int64_t head_stride, int64_t rows, int64_t heads, int bytes) {
+    if (reinterpret_cast<uintptr_t>(p) & 15) return false;
+    return (rows <= 1 || tok_stride * bytes % 16 == 0) && (heads <= 1 || head_stride * bytes % 16 == 0);
+}
+
+}  // namespace
+
+int step_mrope_append(Pool* p, int32_t layer, const gkv_qkv_io* io, int32_t n_tok, int32_t n_heads,
+                      const int32_t* d_positions, int64_t pos_stride, const gkv_mrope_desc* rope,
+                      const gkv_qkv_prologue* pro, cudaStream_t st) {
+    StepWorkspace& ws = p->ws;
+    if (!ws.uploaded) return set_error(GKV_ESTATE, "no step uploaded (call gkv_upload_step or gkv_step_build first)");
+    if (!io || !rope) return set_error(GKV_EINVAL, "qkv/rope description is NULL");
+    const int32_t hk = p->desc.heads_kv, d = p->desc.head_dim, dv = p->desc.v_head_dim;
+    if (layer < 0 || layer >= p->desc.layers)
+        return set_error(GKV_EINVAL, "layer %d outside [0, %d)", layer, p->desc.layers);
+    if (n_heads <= 0 || n_heads % hk != 0)
+        return set_error(GKV_EINVAL, "n_heads %d is not a positive multiple of heads_kv %d", n_heads, hk);
+    if (!valid_q_dtype(io->dtype) || !valid_q_dtype(io->out_dtype))
+        return set_error(GKV_EINVAL, "dtype %d / out_dtype %d is not GKV_DTYPE_F32, GKV_DTYPE_BF16 or GKV_DTYPE_F16", io->dtype,
+                         io->out_dtype);
+    const int32_t R = rope->rope_dim == 0 ? d : rope->rope_dim;
+    if (rope->style != GKV_ROPE_NEOX && rope->style != GKV_ROPE_INTERLEAVED)
+        return set_error(GKV_EINVAL, "rope style %d is neither GKV_ROPE_NEOX nor GKV_ROPE_INTERLEAVED", rope->style);
+    if (R < 0 || R > d || (R & 1)) return set_error(GKV_EINVAL, "rope_dim %d must be even and within [0, head_dim %d]", R, d);
+    if ((d != 32 && d != 64 && d != 128 && d != 256) || dv % 8 != 0 || R % 16 != 0)
+        return set_error(GKV_EUNSUPPORTED, "multi-axis rope append not built for head_dim %d / v_head_dim %d / rope_dim %d", d, dv, R);
+    if (rope->n_axes < 1 || rope->n_axes > GKV_MROPE_MAX_AXES)
+        return set_error(GKV_EINVAL, "n_axes %d outside [1, %d]", rope->n_axes, GKV_MROPE_MAX_AXES);
+    if (R > 0 && (!rope->h_inv_freq || !rope->h_axis)) return set_error(GKV_EINVAL, "inv_freq/axis table is NULL");
+    for (int32_t i = 0; i < R / 2; ++i)
+        if (rope->h_axis[i] >= rope->n_axes)
+            return set_error(GKV_EINVAL, "axis[%d] = %d outside [0, %d)", i, rope->h_axis[i], rope->n_axes);
+    // static layout: the step's own row count, read on the device; the arrays hold n_tok rows
+    if (n_tok < 0 || (!ws.static_mode && n_tok > ws.n_tok))
+        return set_error(GKV_EINVAL, "n_tok %d outside the step's slot mapping [0, %d]", n_tok, ws.n_tok);
+    if (ws.static_mode && n_tok < ws.n_tok)
+        return set_error(GKV_EINVAL, "the static step may have %d rows, the arrays hold %d", ws.n_tok, n_tok);
+    if (n_tok > 0) {
+        if (!io->d_q || !io->d_k || !io->d_v || !io->d_q_out || !d_positions)
+            return set_error(GKV_EINVAL, "q/k/v/q_out/positions is NULL");
+        if (rope->n_axes > 1 && pos_stride < n_tok)
+            return set_error(GKV_EINVAL, "pos_stride %lld below n_tok %d", static_cast<long long>(pos_stride), n_tok);
+        const int eb = elem_bytes_of(io->dtype);
+        if (!rows_aligned(io->d_q, io->q_tok_stride, io->q_head_stride, n_tok, n_heads, eb) ||
+            !rows_aligned(io->d_k, io->k_tok_stride, io->k_head_stride, n_tok, hk, eb) ||
+            !rows_aligned(io->d_v, io->v_tok_stride, io->v_head_stride, n_tok, hk, eb) ||
+            ((reinterpret_cast<uintptr_t>(io->d_q_out) | reinterpret_cast<uintptr_t>(io->d_k_out) |
+              reinterpret_cast<uintptr_t>(io->d_v_out)) & 15))
+            return set_error(GKV_EINVAL, "q/k/v and the outputs need head rows on 16-byte boundaries");
+        const bool in_place = io->d_q_out == io->d_q && io->out_dtype == io->dtype && (n_heads == 1 || io->q_head_stride == d) &&
+                              (n_tok == 1 || io->q_tok_stride == static_cast<int64_t>(n_heads) * d);
+        const void* in[] = {io->d_q, io->d_k, io->d_v};
+        const void* out[] = {io->d_q_out, io->d_k_out, io->d_v_out};
+        for (int i = 0; i < 3; ++i)
+            for (int o = 0; o < 3; ++o)
+                if (out[o] && out[o] == in[i] && !(i == 0 && o == 0 && in_place))
+                    return set_error(GKV_EINVAL, "an output is at the address of an input");
+        if ((out[1] && out[1] == out[0]) || (out[2] && (out[2] == out[0] || out[2] == out[1])))
+            return set_error(GKV_EINVAL, "two outputs share an address");
+    }
+    int rc = static_guard(p);
+    if (rc != GKV_OK) return rc;
+    rc = p->flush_copies(st);
+    if (rc != GKV_OK) return rc;
+    if (n_tok == 0) return GKV_OK;
+    MropeParams a{};
+    a.layer = layer;
+    a.q = io->d_q;
+    a.k = io->d_k;
+    a.v = io->d_v;
+    a.q_out = io->d_q_out;
+    a.k_out = io->d_k_out;
+    a.v_out = io->d_v_out;
+    a.q_ts = io->q_tok_stride;
+    a.q_hs = io->q_head_stride;
+    a.k_ts = io->k_tok_stride;
+    a.k_hs = io->k_head_stride;
+    a.v_ts = io->v_tok_stride;
+    a.v_hs = io->v_head_stride;
+    a.in_dtype = io->dtype;
+    a.out_dtype = io->out_dtype;
+    a.n_tok = ws.static_mode ? std::min(n_tok, ws.max_tokens) : n_tok;
+    a.n_heads = n_heads;
+    a.dyn_tok = ws.static_mode ? reinterpret_cast<const int32_t*>(ws.d_meta[0]) + kHdrTok : nullptr;
+    a.positions = d_positions;
+    a.pos_stride = pos_stride;
+    a.rope_dim = R;
+    a.style = rope->style;
+    a.mscale = rope->mscale == 0.f ? 1.f : rope->mscale;
+    if (pro) {
+        a.q_bias = pro->d_q_bias;
+        a.k_bias = pro->d_k_bias;
+        a.v_bias = pro->d_v_bias;
+        a.q_norm = pro->d_q_norm;
+        a.k_norm = pro->d_k_norm;
+        a.eps = pro->eps;
+    }
+    a.slots = ws.d_slots;
+    a.err = ws.d_err;
+    if (R > 0) {
+        memcpy(a.inv_freq, rope->h_inv_freq, static_cast<size_t>(R / 2) * 4);
+        memcpy(a.axis, rope->h_axis, static_cast<size_t>(R / 2));
+    }
+    if (a.n_tok == 0) return GKV_OK;
+    cudaError_t e = launch_mrope_append(p->geom, a, st);
+    if (e != cudaSuccess) return cuda_fail(e, "mrope_append launch");
+    ws.built = false;
+    p->last_launches += 1;
+    return GKV_OK;
+}
+
+int step_prompt(Pool* p, const gkv_prompt_desc* r, cudaStream_t st) {
+    StepWorkspace& ws = p->ws;
+    if (!r) return set_error(GKV_EINVAL, "prompt description is NULL");
+    const int32_t hk = p->desc.heads_kv, d = p->desc.head_dim, dv = p->desc.v_head_dim;
+    if (r->batch < 0 || r->total < 0) return set_error(GKV_EINVAL, "negative batch %d / total %d", r->batch, r->total);
+    if (r->n_heads <= 0 || r->n_heads % hk != 0)
+        return set_error(GKV_EINVAL, "n_heads %d is not a positive multiple of heads_kv %d", r->n_heads, hk);
+    if (!valid_q_dtype(r->dtype))
+        return set_error(GKV_EINVAL, "dtype %d is not GKV_DTYPE_F32, GKV_DTYPE_BF16 or GKV_DTYPE_F16", r->dtype);
+    if (!std::isfinite(r->scale)) return set_error(GKV_EINVAL, "scale is not finite");
+    if (d % 8 != 0 || dv % 8 != 0 || d > 256 || dv > 256)
+        return set_error(GKV_EUNSUPPORTED, "prompt attention not built for head_dim %d / v_head_dim %d", d, dv);
+    if (r->batch == 0 || r->total == 0) return GKV_OK;
+    if (!r->d_q || !r->d_k || !r->d_v || !r->d_out || !r->d_cu_seqlens)
+        return set_error(GKV_EINVAL, "q/k/v/out/cu_seqlens is NULL");
+    const int eb = elem_bytes_of(r->dtype);
+    if (!rows_aligned(r->d_q, r->q_tok_stride, r->q_head_stride, r->total, r->n_heads, eb) ||
+        !rows_aligned(r->d_k, r->k_tok_stride, r->k_head_stride, r->total, hk, eb) ||
+        !rows_aligned(r->d_v, r->v_tok_stride, r->v_head_stride, r->total, hk, eb) || (reinterpret_cast<uintptr_t>(r->d_out) & 15))
+        return set_error(GKV_EINVAL, "q/k/v and out need head rows on 16-byte boundaries");
+    if (r->d_out == r->d_q || r->d_out == r->d_k || r->d_out == r->d_v)
+        return set_error(GKV_EINVAL, "out is at the address of an input");
+    if ((static_cast<int64_t>(r->total) / 64 + r->batch) * r->n_heads > 0x7fffffff)
+        return set_error(GKV_EINVAL, "%d rows of %d heads exceed the supported size", r->total, r->n_heads);
+    PromptArgs a{};
+    a.q = r->d_q;
+    a.k = r->d_k;
+    a.v = r->d_v;
+    a.out = r->d_out;
+    a.lse = r->d_lse;
+    a.sinks = r->d_sinks;
+    a.cu = r->d_cu_seqlens;
+    a.q_ts = r->q_tok_stride;
+    a.q_hs = r->q_head_stride;
+    a.k_ts = r->k_tok_stride;
+    a.k_hs = r->k_head_stride;
+    a.v_ts = r->v_tok_stride;
+    a.v_hs = r->v_head_stride;
+    a.batch = r->batch;
+    a.total = r->total;
+    a.n_heads = r->n_heads;
+    a.heads_kv = hk;
+    a.d = d;
+    a.dv = dv;
+    a.dtype = r->dtype;
+    a.scale = r->scale;
+    a.err = ws.d_err;
+    cudaError_t e = launch_prompt_simt(a, st);
+    if (e != cudaSuccess) return cuda_fail(e, "prompt_attention launch");
+    ws.built = false;
     p->last_launches += 1;
     return GKV_OK;
 }
@@ -1038,6 +1299,13 @@ int gkv_upload_step(gkv_pool* pool, const int32_t* h_block_tables, int32_t batch
     gkv::DeviceGuard guard(pool->impl.desc.device);
     return gkv::step_upload(&pool->impl, h_block_tables, batch, max_blocks, h_ctx_lens,
                             h_slot_mapping, n_tok, static_cast<cudaStream_t>(stream));
+}
+
+int gkv_step_build(gkv_pool* pool, const gkv_step_io* io, int32_t batch, void* stream) {
+    GKV_DEVICE_POOL(pool);
+    gkv::DeviceGuard guard(pool->impl.desc.device);
+    pool->impl.last_launches = 0;
+    return gkv::step_build(&pool->impl, io, batch, static_cast<cudaStream_t>(stream));
 }
 
 int gkv_upload_step_tables(gkv_pool* pool, gkv_table* const* tables, int32_t batch,
@@ -1219,6 +1487,47 @@ int gkv_rope_inv_freq(float freq_base, int32_t rope_dim, const float* h_freq_fac
     return GKV_OK;
 }
 
+int gkv_mrope_append(gkv_pool* pool, int32_t layer, const gkv_qkv_io* io, int32_t n_tok, int32_t n_heads,
+                     const int32_t* d_positions, int64_t pos_stride, const gkv_mrope_desc* rope,
+                     const gkv_qkv_prologue* prologue, void* stream) {
+    GKV_DEVICE_POOL(pool);
+    gkv::DeviceGuard guard(pool->impl.desc.device);
+    pool->impl.last_launches = 0;
+    return gkv::step_mrope_append(&pool->impl, layer, io, n_tok, n_heads, d_positions, pos_stride, rope, prologue,
+                                  static_cast<cudaStream_t>(stream));
+}
+
+int gkv_mrope_axes(const int32_t* sections, int32_t n_axes, int32_t rope_dim, int32_t interleaved, uint8_t* out) {
+    if (rope_dim < 0 || (rope_dim & 1) || rope_dim > GKV_MROPE_MAX_DIM || n_axes < 1 || n_axes > GKV_MROPE_MAX_AXES || !sections ||
+        (rope_dim > 0 && !out))
+        return set_error(GKV_EINVAL, "sections/out is NULL, or rope_dim %d / n_axes %d out of range", rope_dim, n_axes);
+    int64_t sum = 0;
+    for (int32_t a = 0; a < n_axes; ++a) {
+        if (sections[a] < 0) return set_error(GKV_EINVAL, "sections[%d] = %d is negative", a, sections[a]);
+        sum += sections[a];
+    }
+    if (sum != rope_dim / 2)
+        return set_error(GKV_EINVAL, "sections sum to %lld, not rope_dim / 2 = %d", static_cast<long long>(sum), rope_dim / 2);
+    if (interleaved) {
+        for (int32_t i = 0; i < rope_dim / 2; ++i) {
+            const int32_t a = i % n_axes;
+            out[i] = static_cast<uint8_t>(i < static_cast<int64_t>(n_axes) * sections[a] ? a : 0);
+        }
+    } else {
+        int32_t i = 0;
+        for (int32_t a = 0; a < n_axes; ++a)
+            for (int32_t k = 0; k < sections[a]; ++k) out[i++] = static_cast<uint8_t>(a);
+    }
+    return GKV_OK;
+}
+
+int gkv_prompt_attention(gkv_pool* pool, const gkv_prompt_desc* prompt, void* stream) {
+    GKV_DEVICE_POOL(pool);
+    gkv::DeviceGuard guard(pool->impl.desc.device);
+    pool->impl.last_launches = 0;
+    return gkv::step_prompt(&pool->impl, prompt, static_cast<cudaStream_t>(stream));
+}
+
 int gkv_wait_host_outputs(gkv_pool* pool, void* stream) {
     GKV_DEVICE_POOL(pool);
     Pool& P = pool->impl;
@@ -1290,7 +1599,7 @@ int gkv_sync(gkv_pool* pool, void* stream, int32_t timeout_ms) {
             // a decode that stopped early may leave merge counters raised: start clean
             if (pool->impl.ws.d_merge_count)
                 cudaMemset(pool->impl.ws.d_merge_count, 0, pool->impl.ws.merge_count_cap * sizeof(int32_t));
-            return set_error(GKV_EDEVICE, "a kernel reported error bits 0x%x (1 = bad block id, 2 = wait timeout, 4 = bad slot)", flag);
+            return set_error(GKV_EDEVICE, "a kernel reported error bits 0x%x (1 = bad block id, 2 = wait timeout, 4 = bad slot, 8 = request left out of a built step)", flag);
         }
     }
     return GKV_OK;

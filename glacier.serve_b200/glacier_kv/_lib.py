@@ -91,6 +91,47 @@ class gkv_qkv_prologue(C.Structure):
     ]
 
 
+class gkv_step_io(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("d_ctx_lens", "d_new_lens", "d_new_blocks", "d_block_tables", "d_ctx_out",
+                                          "d_cu_new", "d_slots", "d_positions", "d_counts")] + [
+        ("n_new_blocks", C.c_int32),
+        ("table_stride", C.c_int32),
+        ("max_tokens", C.c_int32),
+    ]
+
+
+class gkv_mrope_desc(C.Structure):
+    _fields_ = [
+        ("rope_dim", C.c_int32),
+        ("style", C.c_int32),
+        ("n_axes", C.c_int32),
+        ("mscale", C.c_float),
+        ("h_inv_freq", C.c_void_p),
+        ("h_axis", C.c_void_p),
+    ]
+
+
+_QKV_STRIDES = [(n, C.c_int64) for n in ("q_tok_stride", "q_head_stride", "k_tok_stride", "k_head_stride", "v_tok_stride",
+                                         "v_head_stride")]
+
+
+class gkv_qkv_io(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("d_q", "d_k", "d_v", "d_q_out", "d_k_out", "d_v_out")] + _QKV_STRIDES + [
+        ("dtype", C.c_int32),
+        ("out_dtype", C.c_int32),
+    ]
+
+
+class gkv_prompt_desc(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("d_q", "d_k", "d_v", "d_out", "d_lse", "d_sinks", "d_cu_seqlens")] + _QKV_STRIDES + [
+        ("batch", C.c_int32),
+        ("total", C.c_int32),
+        ("n_heads", C.c_int32),
+        ("dtype", C.c_int32),
+        ("scale", C.c_float),
+    ]
+
+
 class gkv_pool_stats(C.Structure):
     _fields_ = [
         ("total_blocks", C.c_int32),
@@ -149,6 +190,11 @@ SIGNATURES = {
     "gkv_step_set_static": (C.c_int, [P, I32]),
     "gkv_upload_step": (C.c_int, [P, P, I32, I32, P, P, I32, P]),
     "gkv_upload_step_tables": (C.c_int, [P, P, I32, P, P, I32, P]),
+    "gkv_step_build": (C.c_int, [P, C.POINTER(gkv_step_io), I32, P]),
+    "gkv_mrope_append": (C.c_int, [P, I32, C.POINTER(gkv_qkv_io), I32, I32, P, I64, C.POINTER(gkv_mrope_desc),
+                                   C.POINTER(gkv_qkv_prologue), P]),
+    "gkv_mrope_axes": (C.c_int, [P, I32, I32, I32, P]),
+    "gkv_prompt_attention": (C.c_int, [P, C.POINTER(gkv_prompt_desc), P]),
     "gkv_kv_append": (C.c_int, [P, I32, P, P, I32, P]),
     "gkv_paged_decode": (C.c_int, [P, I32, P, P, I32, F32, P, P]),
     "gkv_rope_append": (C.c_int, [P, I32, P, P, P, I32, I32, P, C.POINTER(gkv_rope_desc),

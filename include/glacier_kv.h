@@ -246,6 +246,40 @@ GKV_API int gkv_upload_step(gkv_pool* pool, const int32_t* h_block_tables, int32
 GKV_API int gkv_upload_step_tables(gkv_pool* pool, gkv_table* const* tables, int32_t batch,
                                    const int32_t* h_ctx_lens, const int64_t* h_slot_mapping,
                                    int32_t n_tok, void* stream);
+/* Device arrays of gkv_step_build. */
+typedef struct gkv_step_io {
+    const int32_t* d_ctx_lens;     /* [batch] tokens each request has stored                      */
+    const int32_t* d_new_lens;     /* [batch] tokens the step adds to it (0: none)                */
+    const int32_t* d_new_blocks;   /* [n_new_blocks] ids for the pages the step opens             */
+    int32_t* d_block_tables;       /* [batch][table_stride], the opened pages' entries are written */
+    int32_t* d_ctx_out;            /* [batch] tokens stored after the step, or NULL               */
+    int32_t* d_cu_new;             /* [batch + 1] first row of each request, or NULL              */
+    int64_t* d_slots;              /* [max_tokens] slot of each row, or NULL                      */
+    int32_t* d_positions;          /* [max_tokens] position of each row in its request, or NULL   */
+    int32_t* d_counts;             /* [2] rows of the step, new blocks used; or NULL              */
+    int32_t n_new_blocks, table_stride, max_tokens;
+} gkv_step_io;
+/* The step's metadata built on the GPU from the requests' lengths, in one launch and with no
+ * copy from the host: in place of gkv_upload_step in the static step layout (GKV_ESTATE
+ * otherwise), and capturable with the launches that follow it, so that a replayed decode needs
+ * only the arrays of `io` rewritten (their addresses and counts are fixed at capture).
+ * Request b has c = ctx_lens[b] tokens stored and adds n = new_lens[b]:
+ *   - pages ceil(c / block_size) .. ceil((c + n) / block_size) - 1 of its table take the next ids
+ *     of new_blocks, requests in order (the host allocates them, e.g. by gkv_table_append_token);
+ *     earlier entries are read, never written;
+ *   - its rows are cu_new[b] .. cu_new[b + 1] - 1 of the step, at positions c, c + 1, ... and the
+ *     slots of their pages.  Entries of d_slots and d_positions behind the last row are left alone;
+ *   - the step's context is c + n (0 tokens: skipped by the decode), and the split-KV work list is
+ *     the one gkv_upload_step builds.
+ * The tables stay the caller's: the step's launches read d_block_tables, which must not change
+ * until they have run.  A request is left out of the step (slots -1, decode output untouched, table
+ * and ctx_out as before, GKV_EDEVICE from the next gkv_sync) when a length is negative, c + n
+ * exceeds table_stride * block_size, its pages need more than n_new_blocks ids or its rows more
+ * than max_tokens.  A block id outside the pool gives slot -1 and GKV_EDEVICE.  batch is at most
+ * the reservation's and 4096, max_tokens at most the reservation's; d_ctx_out must not overlap
+ * d_ctx_lens or d_new_lens.  No reference counterpart (the reference packs tables on the host,
+ * CudaPagedTransformerRunner.cs:367-379). */
+GKV_API int gkv_step_build(gkv_pool* pool, const gkv_step_io* io, int32_t batch, void* stream);
 /* KV append (reshape-and-cache scatter) of the uploaded step's n_tok tokens:
  * d_k [n_tok][heads_kv][head_dim], d_v [n_tok][heads_kv][v_head_dim] fp32, into `layer`.
  * Replaces the per-sequence Store calls, PagedTransformerRunner.cs:634 /
@@ -293,6 +327,86 @@ GKV_API int gkv_rope_append(gkv_pool* pool, int32_t layer, float* d_q, const flo
  * i < rope_dim/2.  Host only. */
 GKV_API int gkv_rope_inv_freq(float freq_base, int32_t rope_dim, const float* h_freq_factors,
                               float* out);
+/* Rotary positions with several axes (time, height and width of images and video). */
+enum { GKV_MROPE_MAX_AXES = 4, GKV_MROPE_MAX_DIM = 256 };
+typedef struct gkv_mrope_desc {
+    int32_t rope_dim;              /* rotated dims per head: even, <= head_dim; 0 = head_dim      */
+    int32_t style;                 /* GKV_ROPE_NEOX or GKV_ROPE_INTERLEAVED (pairing of dims)     */
+    int32_t n_axes;                /* 1 .. GKV_MROPE_MAX_AXES                                     */
+    float mscale;                  /* multiplies the rotated q and k; 0 means 1                   */
+    const float* h_inv_freq;       /* [rope_dim/2] frequencies (gkv_rope_inv_freq)                */
+    const uint8_t* h_axis;         /* [rope_dim/2] position axis of each (gkv_mrope_axes)         */
+} gkv_mrope_desc;
+/* The projections of a step and where the results go.  Row t, head h, element e of q is
+ * d_q[t * q_tok_stride + h * q_head_stride + e] (strides in elements), so the parts of one fused
+ * projection need no copy. */
+typedef struct gkv_qkv_io {
+    const void* d_q;               /* [n_tok][n_heads][head_dim]                                  */
+    const void* d_k;               /* [n_tok][heads_kv][head_dim]                                 */
+    const void* d_v;               /* [n_tok][heads_kv][v_head_dim]                               */
+    void* d_q_out;                 /* dense [n_tok][n_heads][head_dim], rotated; may be d_q where
+                                      that is dense and of the same type                          */
+    void* d_k_out;                 /* dense [n_tok][heads_kv][head_dim], rotated, or NULL         */
+    void* d_v_out;                 /* dense [n_tok][heads_kv][v_head_dim], biased, or NULL        */
+    int64_t q_tok_stride, q_head_stride, k_tok_stride, k_head_stride, v_tok_stride, v_head_stride;
+    int32_t dtype;                 /* of q, k, v: GKV_DTYPE_F32, _BF16 or _F16                    */
+    int32_t out_dtype;             /* of the outputs: GKV_DTYPE_F32, _BF16 or _F16                */
+} gkv_qkv_io;
+/* gkv_rope_append with several position axes, positions on the device, projections of any
+ * GKV_DTYPE_* but FP8 with strides, and outputs beside the arena.  Row t of the step at
+ * positions d_positions[a * pos_stride + t] on axis a: bias, per-head RMSNorm of q and k, then pair
+ * i turned by the angle position(axis[i]) * inv_freq[i] (formed and reduced in 64 bits, so far
+ * positions keep their angle), times mscale; k and v go to their slots in `layer` (rounded once,
+ * from 32 bits, to the arena's type), q to d_q_out, and k and v to d_k_out / d_v_out where given,
+ * for gkv_prompt_attention.  Formulas and `prologue` as gkv_rope_append's; rows with slot -1 are
+ * not stored but their outputs are written.  In the static step layout the rows are the step's own
+ * count, read on the device, and the launch can be captured: n_tok is then the arrays' capacity (at
+ * least the step's max_tokens; rows past it in a later replayed step are left out).  Rows behind the
+ * step's last are left alone.  head_dim must be 32, 64, 128 or 256
+ * (GKV_EUNSUPPORTED).  Element strides and pointers must keep every head row 16-byte aligned, and
+ * d_q_out may only overlap d_q as said above, the other outputs no input (GKV_EINVAL for the
+ * alignment, and for an output at the address of another tensor). */
+GKV_API int gkv_mrope_append(gkv_pool* pool, int32_t layer, const gkv_qkv_io* io, int32_t n_tok,
+                             int32_t n_heads, const int32_t* d_positions, int64_t pos_stride,
+                             const gkv_mrope_desc* rope, const gkv_qkv_prologue* prologue,
+                             void* stream);
+/* The axis table of a rotation whose rope_dim/2 frequencies are shared out by `sections`
+ * ([n_axes], their sum rope_dim/2): one section after the other, or (interleaved != 0) frequency i
+ * to axis i % n_axes as long as i < n_axes * sections[i % n_axes], the rest to axis 0.  Host only. */
+GKV_API int gkv_mrope_axes(const int32_t* sections, int32_t n_axes, int32_t rope_dim,
+                           int32_t interleaved, uint8_t* out);
+/* Whole prompts of different lengths, packed: request b has rows d_cu_seqlens[b] ..
+ * d_cu_seqlens[b + 1] - 1.  Strides in elements, as in gkv_qkv_io. */
+typedef struct gkv_prompt_desc {
+    const void* d_q;               /* [total][n_heads][head_dim]                                  */
+    const void* d_k;               /* [total][heads_kv][head_dim]                                 */
+    const void* d_v;               /* [total][heads_kv][v_head_dim]                               */
+    void* d_out;                   /* dense [total][n_heads][v_head_dim], of the inputs' type     */
+    float* d_lse;                  /* [total][n_heads] ln of the softmax denominator, or NULL     */
+    const float* d_sinks;          /* [n_heads] sink logits, or NULL                              */
+    const int32_t* d_cu_seqlens;   /* [batch + 1], non-decreasing, from 0 to at most total        */
+    int64_t q_tok_stride, q_head_stride, k_tok_stride, k_head_stride, v_tok_stride, v_head_stride;
+    int32_t batch, total;          /* requests; rows of the arrays                                */
+    int32_t n_heads;
+    int32_t dtype;                 /* of q, k, v, out: GKV_DTYPE_F32, _BF16 or _F16               */
+    float scale;
+} gkv_prompt_desc;
+/* Causal attention of whole prompts over their own keys and values, read from the projections
+ * (gkv_mrope_append's outputs) and not from the arena: row t of a request is
+ * softmax(scale * q_t . k_s [, sink]) . v_s over its rows s <= t, query head h reading kv head
+ * h / (n_heads / heads_kv).  Beside gkv_paged_prefill, which reads the arena in its storage type
+ * and lengths from the host, this one takes lengths on the device (d_cu_new of gkv_step_build),
+ * runs in both step layouts and in a captured graph, and offers sinks and lse.  heads_kv, head_dim
+ * and v_head_dim are the pool's; the arena's type does not matter.  16-bit types with head_dim =
+ * v_head_dim = 64 or 128 and scale > 0 run on the tensor cores (p rounded to the inputs' type
+ * before p . v), the others in 32-bit arithmetic; softmax statistics are 32 bits.  Masked keys and
+ * values, and rows of other requests, never reach a result, whatever they hold.  Rows behind
+ * cu_seqlens[batch] are left alone.  A prompt whose range is negative or passes `total` is left out
+ * (GKV_EDEVICE from the next gkv_sync).  head_dim and v_head_dim must be multiples of 8 and at most
+ * 256 (GKV_EUNSUPPORTED); element strides and pointers must keep every head row 16-byte aligned
+ * (GKV_EINVAL).  d_out and d_lse must not overlap the inputs.  Replaces, for a fresh prompt, the
+ * per-token loop of PagedTransformerRunner.ForwardPrefillSubBatch (PagedTransformerRunner.cs:424-471). */
+GKV_API int gkv_prompt_attention(gkv_pool* pool, const gkv_prompt_desc* prompt, void* stream);
 /* Split-KV GQA paged decode of the uploaded step for `layer`:
  * d_q [batch][n_heads][head_dim] fp32 -> d_out [batch][n_heads][v_head_dim] fp32.
  * out = softmax(scale * q.K^T [, sink]) . V over each sequence's ctx_len tokens, query
