@@ -139,9 +139,12 @@ def _f32_dev(t, name: str):
 
 
 class _CudaArray:
-    """__cuda_array_interface__ wrapper so torch can view the device arena in place."""
+    """__cuda_array_interface__ wrapper so torch can view the device arena in place.  A tensor made
+    from it holds it, and it holds the pool: an arena whose views are alive is not freed with the
+    last other reference to its pool (close() still frees it at once)."""
 
-    def __init__(self, ptr: int, shape: Tuple[int, ...], typestr: str):
+    def __init__(self, ptr: int, shape: Tuple[int, ...], typestr: str, owner: "PagedBlockPool"):
+        self.owner = owner
         self.__cuda_array_interface__ = {
             "shape": tuple(shape), "typestr": typestr, "data": (ptr, False), "version": 3,
             "strides": None,
@@ -275,11 +278,11 @@ class PagedBlockPool:
             raise InvalidOperationError(GKV_ESTATE, "Host KV buffers were omitted.")
         shape = (self.total_blocks, self._layers, self._heads_kv, self.block_size, dim)
         if self.dtype == "fp8":
-            return torch.as_tensor(_CudaArray(ptr, shape, "|u1"), device=f"cuda:{self.device}")
+            return torch.as_tensor(_CudaArray(ptr, shape, "|u1", self), device=f"cuda:{self.device}")
         if self.dtype in ("bf16", "f16"):
-            t = torch.as_tensor(_CudaArray(ptr, shape, "<i2"), device=f"cuda:{self.device}")
+            t = torch.as_tensor(_CudaArray(ptr, shape, "<i2", self), device=f"cuda:{self.device}")
             return t.view(torch.bfloat16 if self.dtype == "bf16" else torch.float16)
-        return torch.as_tensor(_CudaArray(ptr, shape, "<f4"), device=f"cuda:{self.device}")
+        return torch.as_tensor(_CudaArray(ptr, shape, "<f4", self), device=f"cuda:{self.device}")
 
     # ---- allocator, PagedBlockPool.cs:178-353 ----
     def try_allocate_block(self) -> Tuple[bool, int]:

@@ -250,3 +250,20 @@ def test_queued_forks_run_before_the_next_append(cuda):
     assert pool.last_launch_count == 2  # the flushed fork + the append
     col = pool.key_view()[blk, 0, 0, :6, 0].tolist()
     assert col == [0.0, 1.0, 2.0, 3.0, 4.0, 55.0]
+
+
+def test_arena_views_keep_their_pool(cuda):
+    """A view of the arena outlives the last other reference to its pool."""
+    import gc
+    import weakref
+
+    pool = G.PagedBlockPool(4, 1, 1, 32, 16)
+    alive = weakref.ref(pool)
+    view = pool.key_view()
+    part = view[1:, 0].reshape(-1)[:5]
+    del pool, view
+    gc.collect()
+    assert alive() is not None and float(part.sum()) == 0.0
+    del part
+    gc.collect()
+    assert alive() is None
