@@ -146,6 +146,8 @@ struct PromptArgs {
     int* err;
 };
 cudaError_t launch_prompt_simt(const PromptArgs& a, cudaStream_t st);
+// The tensor-core kernel, where type, head dims, scale and strides allow it (*ran says whether).
+cudaError_t launch_prompt_tc(const PromptArgs& a, bool* ran, cudaStream_t st);
 
 // ---- block copy ----
 // ops: [n][3] int32 (src, dst, valid_tokens) in device memory.

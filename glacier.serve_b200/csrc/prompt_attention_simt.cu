@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(kThreads) prompt_simt_kernel(const PromptArgs 
     float* sP = sV + kN * LD;  // [kM][kN + 4]
     constexpr int LP = kN + 4;
     const int x = blockIdx.x / a.n_heads, head = blockIdx.x - x * a.n_heads;
-    if (blockIdx.x == 0) check_prompts(a);
+    if (blockIdx.x == 0) check_prompts(a, threadIdx.x, kThreads);
     PromptTile pt;
     if (!find_prompt_tile<kM>(a, static_cast<int>(gridDim.x / a.n_heads) - 1 - x, pt)) return;
     const int hkv = head / (a.n_heads / a.heads_kv);

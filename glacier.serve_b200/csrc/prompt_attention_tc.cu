@@ -1,0 +1,595 @@
+// Causal attention of packed prompts on the 5th-generation tensor cores (tcgen05, accumulators in
+// tensor memory): 16-bit types, head_dim = v_head_dim = 64 or 128.
+//
+//   out_t = sum_{s <= t} p_ts v_s / l_t,  p_ts = 2^(c q_t . k_s - m_t),  c = scale log2 e,
+//   l_t = sum_s p_ts [+ 2^(sink log2 e - m_t)],  lse_t = (m_t + log2 l_t) ln 2.
+//
+// A work item is 256 consecutive queries of one (prompt, head), as two tiles of 128 that share every
+// key tile of 128.  Per key tile and query tile: S = Q K^T (M = N = 128) into tensor memory, softmax,
+// P over S in the inputs' type, O += P V.  The two query tiles take turns: while one tile's scores
+// are in its softmax, the tensor pipe runs the other's products, so neither waits for the other as
+// long as both take about the same time (2 * 128^3 products at 4096 a cycle, 128^2 exponentials at
+// 16 a cycle: 1024 cycles each).  Roles:
+//  * warps 0-3 and 4-7, one warpgroup per query tile, one thread per query row: scores from tensor
+//    memory, causal mask on the last key tile, online softmax with lazy rescaling (O is rescaled
+//    only where the running maximum grows by more than 2^8, so p stays below 2^8), P back into tensor
+//    memory; at the end O / l through shared memory to whole rows of the output.
+//  * warp 8: one thread issues every product.  S of key tile j + 1 overwrites P of tile j, so it is
+//    issued behind P V of tile j (products of one thread execute in issue order), and a warpgroup
+//    that sees S of tile j + 1 knows that O holds P V of tile j: rescaling needs no further barrier.
+//  * warp 9: one thread loads Q, and K and V tiles in turn through a ring of 4 slots (TMA, 128-byte
+//    swizzle, no multicast).
+//  * warp 10: finds the next item while the block works on this one.  The grid holds every item, the
+//    longest of a prompt first; a running block takes over blocks that have not started
+//    (clusterlaunchcontrol), so the next item's loads and first scores overlap this one's end.
+// Values that no row may see (keys behind a prompt's end, and not-finite values of keys that some rows
+// of the last key tile do not see) are taken out of the V tile before its product; the rows that do see
+// a not-finite value get it back in the epilogue.
+// Every wait is bounded: on expiry the block raises kErrWaitTimeout, lets its copies and products
+// finish, frees its tensor memory and ends.
+#include <cuda.h>
+
+#include <atomic>
+
+#include "gkv_device.cuh"
+#include "kernels.h"
+#include "prompt_tiles.cuh"
+#include "../../include/glacier_kv.h"
+
+namespace gkv {
+
+namespace {
+
+constexpr int kBM = 128, kBN = 128;               // query rows of a tile, keys of a tile
+constexpr int kRows = 2 * kBM;                    // query rows of an item
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kPlanWarp = 10;
+constexpr int kThreads = 384;
+constexpr int kRing = 4;
+constexpr uint32_t kTmemCols = 512;               // S0 S1 O0 O1, 128 columns each
+constexpr uint32_t kColS = 0, kColO = 256;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRescaleLog2 = 8.f;
+
+template <int D>
+struct Shape {
+    static constexpr uint32_t kHalf = kBN * 128;            // 128 rows x 64 dims
+    static constexpr int kHalves = D / 64;
+    static constexpr uint32_t kTile = kHalves * kHalf;      // a Q, K or V tile
+    static constexpr uint32_t kStage = kBM * 64;            // output staging of a warpgroup: 128 rows x 32 dims
+    static constexpr uint32_t kData = 2 * kTile + kRing * kTile + 2 * kStage;
+    static constexpr uint32_t kBytes = kData + 13312 + 1024;  // + bookkeeping + alignment
+};
+
+struct Item {
+    int64_t row0;   // first row of the prompt
+    int q0, len;    // first query in the prompt, the prompt's length
+    int head;
+    int n[2];       // key tiles of each query tile (0: no rows); n[0] = 0: no further item
+    int number;     // of this block's items
+};
+
+struct Book {
+    uint64_t q_full, q_empty;
+    uint64_t ring_full[kRing], ring_empty[kRing];
+    uint64_t s_full[2], p_full[2], o_full[2];
+    uint64_t item_full, item_empty;
+    uint64_t steal, drained;
+    alignas(16) uint32_t response[4];
+    Item item;
+    uint32_t tmem;
+    int abort;
+    // Not-finite values taken out of a query tile's last key tile: for each dim the first position with
+    // NaN, +infinity, -infinity, under the complement of the item's number, so that a later item's
+    // entries replace an earlier one's.  Two sets, for even and odd items: the first warpgroup may be
+    // one item ahead of the second, which reads both tiles' entries, and not more.
+    int poisoned[2][2];  // one more than the number of the item that the entries are of
+    unsigned long long poison[2][2][3][128];
+};
+static_assert(sizeof(Book) <= 13312, "bookkeeping");
+
+constexpr uint32_t idesc_16(int m, int n, bool b_mn_major, bool f16) {
+    const uint32_t fmt = f16 ? 0u : 1u;
+    return (1u << 4) | (fmt << 7) | (fmt << 10) | ((b_mn_major ? 1u : 0u) << 16) |
+           (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// Bounded wait that also ends (false) when the block has given up.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Book* bk) {
+    const uint32_t addr = smem_u32(bar);
+    for (uint32_t it = 0; it < kWaitLimit; ++it) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(addr), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if ((it & 63) == 63 && *reinterpret_cast<volatile int*>(&bk->abort)) return false;
+    }
+    return false;
+}
+
+// Asks for a block of the grid that has not started; the answer lands in `response`.
+__device__ __forceinline__ void steal_block(uint32_t* response, uint64_t* bar) {
+    mbar_arrive_expect_tx(bar, 16);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                     smem_u32(response)),
+                 "r"(smem_u32(bar))
+                 : "memory");
+}
+// Its number, or -1 when there was none left.
+__device__ __forceinline__ int stolen_block(const uint32_t* response) {
+    uint32_t ok, x;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t"
+        "ld.shared.b128 r, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "mov.u32 %1, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+        : "=r"(ok), "=r"(x)
+        : "r"(smem_u32(response))
+        : "memory");
+    return ok ? static_cast<int>(x) : -1;
+}
+
+template <bool F16>
+__device__ __forceinline__ uint32_t times_zero(uint32_t acc, uint32_t x) {  // acc + 0 * x: NaN where x is not finite
+    if constexpr (F16) {
+        const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(0.f), *reinterpret_cast<const __half2*>(&acc));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    } else {
+        const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x), __float2bfloat162_rn(0.f),
+                                         *reinterpret_cast<const __nv_bfloat162*>(&acc));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+}
+
+// The last key tile of query tile t, in shared memory: thread `key` of the warpgroup takes one key row.
+// Rows behind the prompt become zero; not-finite elements become zero and are noted.
+template <int D, bool F16>
+__device__ __forceinline__ void clean_values(uint8_t* tile, int key, int key_pos, int len, Book* bk, int number, int t) {
+    constexpr uint32_t kInf = F16 ? 0x7c00u : 0x7f80u;
+    if (key_pos >= len) {
+#pragma unroll
+        for (int h = 0; h < Shape<D>::kHalves; ++h)
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+                *reinterpret_cast<uint4*>(tile + h * Shape<D>::kHalf + key * 128 + ((c ^ (key & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+        return;
+    }
+    uint32_t acc = 0;
+#pragma unroll
+    for (int h = 0; h < Shape<D>::kHalves; ++h)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            const uint4 w = *reinterpret_cast<const uint4*>(tile + h * Shape<D>::kHalf + key * 128 + ((c ^ (key & 7)) << 4));
+            acc = times_zero<F16>(acc, w.x);
+            acc = times_zero<F16>(acc, w.y);
+            acc = times_zero<F16>(acc, w.z);
+            acc = times_zero<F16>(acc, w.w);
+        }
+    if ((acc & 0x7fff7fffu) == 0) return;
+    // rare: element by element (chunk c of a row sits at c ^ (row % 8))
+    for (int e = 0; e < D; ++e) {
+        uint8_t* p = tile + (e >> 6) * Shape<D>::kHalf + key * 128 + ((((e & 63) >> 3) ^ (key & 7)) << 4) + (e & 7) * 2;
+        const uint32_t x = *reinterpret_cast<uint16_t*>(p);
+        if ((x & kInf) != kInf) continue;
+        const int kind = (x & 0x7fffu) != kInf ? 0 : (x & 0x8000u) ? 2 : 1;
+        atomicMin(&bk->poison[number & 1][t][kind][e],
+                  (static_cast<unsigned long long>(~static_cast<uint32_t>(number)) << 32) | static_cast<uint32_t>(key_pos));
+        bk->poisoned[number & 1][t] = number + 1;
+        *reinterpret_cast<uint16_t*>(p) = 0;
+    }
+}
+
+template <int D, bool F16>
+__global__ void __launch_bounds__(kThreads, 1)
+    prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
+                     const __grid_constant__ CUtensorMap tmv, const __grid_constant__ PromptArgs a) {
+    using Sh = Shape<D>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t{1023});
+    uint8_t* sQ = smem;
+    uint8_t* sRing = sQ + 2 * Sh::kTile;
+    uint8_t* sStage = sRing + kRing * Sh::kTile;
+    Book* bk = reinterpret_cast<Book*>(smem + Sh::kData);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        mbar_init(&bk->q_full, 1);
+        mbar_init(&bk->q_empty, 1);
+        for (int i = 0; i < kRing; ++i) {
+            mbar_init(&bk->ring_full[i], 1);
+            mbar_init(&bk->ring_empty[i], 1);
+        }
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&bk->s_full[t], 1);
+            mbar_init(&bk->p_full[t], 128);
+            mbar_init(&bk->o_full[t], 1);
+            bk->poisoned[t][0] = bk->poisoned[t][1] = 0;
+        }
+        mbar_init(&bk->item_full, 1);
+        mbar_init(&bk->item_empty, 10);  // both warpgroups' warps, the issuer, the loader
+        mbar_init(&bk->steal, 1);
+        mbar_init(&bk->drained, 1);
+        bk->abort = 0;
+        fence_mbar_init();
+    }
+    for (int i = threadIdx.x; i < 2 * 2 * 3 * 128; i += kThreads) (&bk->poison[0][0][0][0])[i] = ~0ull;
+    if (warp == kMmaWarp) tmem_alloc(&bk->tmem, kTmemCols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bk->tmem;
+    bool ok = true;
+
+    if (warp == kPlanWarp) {
+        // ---------------- items ----------------
+        if (blockIdx.x == 0) check_prompts(a, lane, 32);
+        int block = blockIdx.x, published = 0;
+        uint32_t asked = 0;
+        const int last = static_cast<int>(gridDim.x / a.n_heads) - 1;
+        while (true) {
+            PromptTile pt;
+            const int x = block / a.n_heads;
+            const bool found = block >= 0 && find_prompt_tile<kRows>(a, last - x, pt);
+            if (found || block < 0) {
+                if (lane == 0) {
+                    Item it{};
+                    if (found) {
+                        it.row0 = pt.row0;
+                        it.q0 = pt.tile * kRows;
+                        it.len = pt.len;
+                        it.head = block - x * a.n_heads;
+                        it.n[0] = it.q0 / kBN + 1;
+                        it.n[1] = it.len - it.q0 > kBM ? it.n[0] + 1 : 0;
+                        it.number = published;
+                    }
+                    bk->item = it;
+                    mbar_arrive(&bk->item_full);
+                }
+                __syncwarp();
+                if (block < 0) break;
+                // the next item is fetched once every warp has begun this one
+                if (!(ok = __all_sync(~0u, wait(&bk->item_empty, published & 1, bk)))) break;
+                ++published;
+            }
+            if (lane == 0) steal_block(bk->response, &bk->steal);
+            __syncwarp();
+            if (!(ok = __all_sync(~0u, mbar_wait(&bk->steal, asked & 1)))) break;  // the answer must land, come what may
+            ++asked;
+            block = stolen_block(bk->response);
+            __syncwarp();
+            fence_proxy_async_smem();  // the answer has been read before the next one is written
+        }
+        if (!ok && lane == 0) {
+            bk->abort = 1;
+            atomicOr(a.err, kErrWaitTimeout);
+        }
+    } else if (warp == kLoadWarp) {
+        // ---------------- TMA ----------------
+        if (lane == 0) {
+            uint32_t slot = 0, q_loads = 0;
+            for (uint32_t i = 0;; ++i) {
+                if (!(ok = wait(&bk->item_full, i & 1, bk))) break;
+                const Item it = bk->item;
+                mbar_arrive(&bk->item_empty);
+                if (it.n[0] == 0) break;
+                if (i > 0 && !(ok = wait(&bk->q_empty, (i - 1) & 1, bk))) break;
+                const int kv = it.head / (a.n_heads / a.heads_kv);
+                const int row = static_cast<int>(it.row0) + it.q0;
+                mbar_arrive_expect_tx(&bk->q_full, it.n[1] ? 2 * Sh::kTile : Sh::kTile);
+                ++q_loads;
+                const int nj = it.n[1] ? it.n[1] : it.n[0];
+                auto load = [&](uint8_t* dst, const CUtensorMap* tm, int head, int r, uint64_t* bar) {
+#pragma unroll
+                    for (int h = 0; h < Sh::kHalves; ++h) tma_load_3d(dst + h * Sh::kHalf, tm, h * 64, head, r, bar);
+                };
+                load(sQ, &tmq, it.head, row, &bk->q_full);
+                for (int j = 0; j < 2 * nj; ++j) {  // K of tile j / 2, then V
+                    const int s = slot % kRing;
+                    if (slot >= kRing && !(ok = wait(&bk->ring_empty[s], (slot / kRing - 1) & 1, bk))) break;
+                    mbar_arrive_expect_tx(&bk->ring_full[s], Sh::kTile);
+                    load(sRing + s * Sh::kTile, (j & 1) ? &tmv : &tmk, kv, static_cast<int>(it.row0) + (j >> 1) * kBN, &bk->ring_full[s]);
+                    ++slot;
+                    if (j == 0 && it.n[1]) load(sQ + Sh::kTile, &tmq, it.head, row + kBM, &bk->q_full);
+                }
+                if (!ok) break;
+            }
+            if (!ok) {
+                bk->abort = 1;
+                atomicOr(a.err, kErrWaitTimeout);
+                // every copy must land before the block's shared memory goes away
+                if (q_loads) mbar_wait(&bk->q_full, (q_loads - 1) & 1);
+                for (uint32_t s = slot > kRing ? slot - kRing : 0; s < slot; ++s) mbar_wait(&bk->ring_full[s % kRing], (s / kRing) & 1);
+            }
+        }
+    } else if (warp == kMmaWarp) {
+        // ---------------- products ----------------
+        if (lane == 0) {
+            constexpr uint32_t kIdS = idesc_16(kBM, kBN, false, F16);
+            constexpr uint32_t kIdO = idesc_16(kBM, D, true, F16);
+            uint32_t slot = 0;          // ring position of the next tile
+            uint32_t p_count[2] = {0, 0};
+            auto scores = [&](int t, uint32_t ks) {  // S_t = Q_t K^T
+                const uint32_t q = smem_u32(sQ) + t * Sh::kTile, k = smem_u32(sRing) + ks * Sh::kTile;
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk)
+                    umma_f16(tmem + kColS + t * 128, umma_desc_sw128(q + (kk >> 2) * Sh::kHalf + (kk & 3) * 32, 16, 1024),
+                             umma_desc_sw128(k + (kk >> 2) * Sh::kHalf + (kk & 3) * 32, 16, 1024), kIdS, kk > 0 ? 1u : 0u);
+                umma_commit(&bk->s_full[t]);
+            };
+            for (uint32_t i = 0;; ++i) {
+                if (!(ok = wait(&bk->item_full, i & 1, bk))) break;
+                const int n0 = bk->item.n[0], n1 = bk->item.n[1];
+                mbar_arrive(&bk->item_empty);
+                if (n0 == 0) break;
+                const int n[2] = {n0, n1};
+                const int nj = n1 ? n1 : n0;
+                uint32_t ks = slot % kRing;
+                if (!(ok = wait(&bk->ring_full[ks], (slot / kRing) & 1, bk) && wait(&bk->q_full, i & 1, bk))) break;
+                tc_fence_after();
+                scores(0, ks);
+                if (n1) scores(1, ks);
+                umma_commit(&bk->ring_empty[ks]);
+                if (nj == 1) umma_commit(&bk->q_empty);
+                ++slot;
+                for (int j = 0; ok && j < nj; ++j) {
+                    const uint32_t vs = slot % kRing;
+                    if (!(ok = wait(&bk->ring_full[vs], (slot / kRing) & 1, bk))) break;
+                    ++slot;
+                    const bool more = j + 1 < nj;
+                    ks = slot % kRing;
+                    if (more && !(ok = wait(&bk->ring_full[ks], (slot / kRing) & 1, bk))) break;
+                    slot += more ? 1 : 0;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        if (j >= n[t]) continue;
+                        if (!(ok = wait(&bk->p_full[t], p_count[t] & 1, bk))) break;
+                        ++p_count[t];
+                        tc_fence_after();
+                        const uint32_t v = smem_u32(sRing) + vs * Sh::kTile;
+#pragma unroll
+                        for (int kk = 0; kk < kBN / 16; ++kk)
+                            // V tile [key][dim]: MN-major, 8-key groups 1 KB apart, dims 64-127 in the second half
+                            umma_f16_ts(tmem + kColO + t * 128, tmem + kColS + t * 128 + kk * 8,
+                                        umma_desc_sw128(v + kk * 2048, Sh::kHalf, 1024), kIdO, (j > 0 || kk > 0) ? 1u : 0u);
+                        if (j + 1 < n[t]) scores(t, ks);
+                        else umma_commit(&bk->o_full[t]);
+                    }
+                    if (!ok) break;
+                    umma_commit(&bk->ring_empty[vs]);
+                    if (more) {
+                        umma_commit(&bk->ring_empty[ks]);
+                        if (j + 2 == nj) umma_commit(&bk->q_empty);
+                    }
+                }
+                if (!ok) break;
+            }
+            if (!ok) {
+                bk->abort = 1;
+                atomicOr(a.err, kErrWaitTimeout);
+            }
+            umma_commit(&bk->drained);  // every product is complete before the tensor memory is freed
+            if (!mbar_wait(&bk->drained, 0)) atomicOr(a.err, kErrWaitTimeout);
+        }
+    } else if (warp < 8) {
+        // ---------------- softmax and epilogue ----------------
+        const int t = warp >> 2, r = threadIdx.x & 127;
+        const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+        const uint32_t tS = tmem + kColS + t * 128 + lanes, tO = tmem + kColO + t * 128 + lanes;
+        const float sl = a.scale * kLog2e;
+        uint32_t s_count = 0, o_count = 0;
+        uint32_t slot0 = 0;  // ring position of the item's first tile
+        for (uint32_t i = 0; ok; ++i) {
+            if (!(ok = __all_sync(~0u, wait(&bk->item_full, i & 1, bk)))) break;
+            const Item it = bk->item;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bk->item_empty);
+            if (it.n[0] == 0) break;
+            const int n = t ? it.n[1] : it.n[0];
+            const int nj = it.n[1] ? it.n[1] : it.n[0];
+            const int pos = it.q0 + t * kBM + r;
+            float m_run = -INFINITY, l_run = 0.f;
+            for (int j = 0; j < n; ++j) {
+                if (!(ok = __all_sync(~0u, wait(&bk->s_full[t], s_count & 1, bk)))) break;
+                ++s_count;
+                tc_fence_after();
+                uint32_t s[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, s[c]);
+                tmem_wait_ld();
+                if (j == n - 1) {
+                    const int limit = pos - j * kBN;  // keys 0 .. limit of the tile
+#pragma unroll
+                    for (int c = 0; c < 128; ++c)
+                        if (c > limit) s[c >> 5][c & 31] = 0xff800000u;
+                }
+                float mq[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const uint32_t* x = &s[k >> 1][(k & 1) * 16];
+                    float m = __uint_as_float(x[0]);
+#pragma unroll
+                    for (int e = 1; e < 15; e += 2) m = fmax3(m, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+                    mq[k] = fmaxf(m, __uint_as_float(x[15]));
+                }
+                const float mt = fmax3(fmax3(mq[0], mq[1], mq[2]), fmax3(mq[3], mq[4], mq[5]), fmaxf(mq[6], mq[7])) * sl;
+                const bool need = mt > m_run + kRescaleLog2;
+                float alpha = 1.f;
+                if (need) {
+                    alpha = fast_exp2(m_run - mt);  // 0 on the first tile
+                    m_run = mt;
+                    l_run *= alpha;
+                }
+                if (j > 0 && __any_sync(~0u, need)) {
+                    // O holds P V up to tile j - 1: its products were issued before S of this tile
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t o[32];
+                        tmem_ld32(tO + c * 32, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                        tmem_st32(tO + c * 32, o);
+                    }
+                }
+                const float2 sl2 = make_float2(sl, sl), nm2 = make_float2(-m_run, -m_run);
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const uint32_t* x = &s[2 * c + (e >> 4)][(e & 15) * 2];
+                        const float2 y = __ffma2_rn(make_float2(__uint_as_float(x[0]), __uint_as_float(x[1])), sl2, nm2);
+                        const float2 p = make_float2(fast_exp2(y.x), fast_exp2(y.y));
+                        sum[e & 1] = __fadd2_rn(sum[e & 1], p);
+                        pk[e] = pack_16x2<F16>(p.x, p.y);
+                    }
+                    tmem_st32(tS + c * 32, pk);  // P over the first 64 columns of S
+                }
+                l_run += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                if (j == n - 1) {
+                    const uint32_t vs = slot0 + 2 * j + 1;
+                    if (!(ok = __all_sync(~0u, wait(&bk->ring_full[vs % kRing], (vs / kRing) & 1, bk)))) break;
+                    clean_values<D, F16>(sRing + (vs % kRing) * Sh::kTile, r, j * kBN + r, it.len, bk, it.number, t);
+                    fence_proxy_async_smem();
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(&bk->p_full[t]);
+            }
+            slot0 += 2 * nj;
+            if (!ok || n == 0) continue;
+            if (!(ok = __all_sync(~0u, wait(&bk->o_full[t], o_count & 1, bk)))) break;
+            ++o_count;
+            tc_fence_after();
+            // the sink joins the sum against the larger of the two maxima
+            float inv, top = m_run, total = l_run;
+            if (a.sinks) {
+                const float sink = __ldg(a.sinks + it.head) * kLog2e;
+                top = fmaxf(m_run, sink);
+                const float base = top == -INFINITY ? 0.f : top;
+                const float alpha = fast_exp2(m_run - base);
+                total = l_run * alpha + fast_exp2(sink - base);
+                inv = alpha / total;
+            } else {
+                inv = 1.f / l_run;
+            }
+            const int rows = min(kBM, it.len - it.q0 - t * kBM);
+            const int64_t row = it.row0 + it.q0 + t * kBM;
+            if (a.lse && r < rows) a.lse[(row + r) * a.n_heads + it.head] = (top + log2f(total)) * 0.6931471805599453f;
+            uint8_t* stage = sStage + t * Sh::kStage + (warp & 3) * (32 * 64);
+            uint8_t* out = static_cast<uint8_t*>(a.out) + (row * a.n_heads + it.head) * (D * 2);
+            const int64_t out_row = static_cast<int64_t>(a.n_heads) * (D * 2);
+            const volatile int* tags = bk->poisoned[it.number & 1];
+            const bool bad = tags[0] == it.number + 1 || (t && tags[1] == it.number + 1);
+#pragma unroll 1
+            for (int h = 0; h < D / 32; ++h) {
+                uint32_t o[32];
+                tmem_ld32(tO + h * 32, o);
+                tmem_wait_ld();
+                if (bad) {
+                    // rows that see a not-finite value taken out of the last key tiles: of the own one
+                    // and, for the second query tile, of the first's
+#pragma unroll 1
+                    for (int e = 0; e < 32; ++e) {
+                        bool sees[3];
+                        for (int k = 0; k < 3; ++k) {
+                            sees[k] = false;
+                            for (int u = 0; u <= t; ++u) {
+                                const unsigned long long w = bk->poison[it.number & 1][u][k][h * 32 + e];
+                                sees[k] |= static_cast<uint32_t>(w >> 32) == ~static_cast<uint32_t>(it.number) &&
+                                           static_cast<uint32_t>(pos) >= static_cast<uint32_t>(w);
+                            }
+                        }
+                        float add = 0.f;
+                        if (sees[0] || (sees[1] && sees[2])) add = __uint_as_float(0x7fffffffu);
+                        else if (sees[1]) add = INFINITY;
+                        else if (sees[2]) add = -INFINITY;
+#pragma unroll
+                        for (int q = 0; q < 32; ++q)
+                            if (q == e) o[q] = __float_as_uint(__uint_as_float(o[q]) + add);
+                    }
+                }
+                __syncwarp();  // the last piece's rows have been read from the stage
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        w[e] = pack_16x2<F16>(__uint_as_float(o[c * 8 + e * 2]) * inv, __uint_as_float(o[c * 8 + e * 2 + 1]) * inv);
+                    *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+                __syncwarp();
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int rr = k * 8 + (lane >> 2), c = lane & 3;
+                    const uint4 w = *reinterpret_cast<const uint4*>(stage + rr * 64 + ((c ^ ((rr >> 1) & 3)) << 4));
+                    const int tr = (warp & 3) * 32 + rr;
+                    if (tr < rows) *reinterpret_cast<uint4*>(out + tr * out_row + h * 64 + c * 16) = w;
+                }
+            }
+            tc_fence_before();
+        }
+        if (!ok) {
+            bk->abort = 1;
+            atomicOr(a.err, kErrWaitTimeout);
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kTmemCols);
+    }
+}
+
+template <int D, bool F16>
+cudaError_t launch(const PromptArgs& a, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t st) {
+    static std::atomic<uint64_t> done_mask{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(done_mask.load(std::memory_order_acquire) & bit)) {
+        e = cudaFuncSetAttribute(prompt_tc_kernel<D, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kBytes);
+        if (e != cudaSuccess) return e;
+        done_mask.fetch_or(bit, std::memory_order_acq_rel);
+    }
+    const int64_t grid = prompt_tile_bound(a, kRows) * a.n_heads;
+    if (grid > 0x7fffffff) return cudaErrorInvalidValue;
+    prompt_tc_kernel<D, F16><<<static_cast<unsigned>(grid), kThreads, Shape<D>::kBytes, st>>>(mq, mk, mv, a);
+    return cudaGetLastError();
+}
+
+// [rows][heads][d] with strides, in boxes of 128 rows x 64 dims of one head.
+bool encode(CUtensorMap* m, const void* p, int d, int heads, int64_t rows, int64_t hs, int64_t ts) {
+    const uint64_t dims[3] = {static_cast<uint64_t>(d), static_cast<uint64_t>(heads), static_cast<uint64_t>(rows)};
+    // a stride that is never taken may be anything in the caller's tensor, but not in the map
+    const uint64_t strides[2] = {static_cast<uint64_t>(heads > 1 ? hs : d) * 2, static_cast<uint64_t>(rows > 1 ? ts : d) * 2};
+    const uint32_t box[3] = {64, 1, static_cast<uint32_t>(kBM)};
+    return encode_bf16_map3(m, p, dims, strides, box);
+}
+
+}  // namespace
+
+cudaError_t launch_prompt_tc(const PromptArgs& a, bool* ran, cudaStream_t st) {
+    *ran = false;
+    if (a.dtype == GKV_DTYPE_F32 || a.d != a.dv || (a.d != 64 && a.d != 128) || !(a.scale > 0.f) || !tmap_encoder_available())
+        return cudaSuccess;
+    alignas(64) CUtensorMap mq, mk, mv;
+    if (!encode(&mq, a.q, a.d, a.n_heads, a.total, a.q_hs, a.q_ts) || !encode(&mk, a.k, a.d, a.heads_kv, a.total, a.k_hs, a.k_ts) ||
+        !encode(&mv, a.v, a.d, a.heads_kv, a.total, a.v_hs, a.v_ts))
+        return cudaSuccess;  // strides that a tensor map cannot hold
+    *ran = true;
+    if (a.dtype == GKV_DTYPE_BF16) return a.d == 128 ? launch<128, false>(a, mq, mk, mv, st) : launch<64, false>(a, mq, mk, mv, st);
+    return a.d == 128 ? launch<128, true>(a, mq, mk, mv, st) : launch<64, true>(a, mq, mk, mv, st);
+}
+
+}  // namespace gkv

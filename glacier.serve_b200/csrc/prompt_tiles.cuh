@@ -39,9 +39,9 @@ __device__ __forceinline__ bool find_prompt_tile(const PromptArgs& a, int x, Pro
     return out.tile >= 0 && static_cast<int64_t>(out.tile) * T < out.len;
 }
 
-// A block looks every prompt's range over, whether or not a tile of it is ever searched for.
-__device__ __forceinline__ void check_prompts(const PromptArgs& a) {
-    for (int b = threadIdx.x; b < a.batch; b += blockDim.x) {
+// Looks every prompt's range over, whether or not a tile of it is ever searched for.
+__device__ __forceinline__ void check_prompts(const PromptArgs& a, int first, int step) {
+    for (int b = first; b < a.batch; b += step) {
         const int begin = __ldg(a.cu + b), end = __ldg(a.cu + b + 1);
         if (begin < 0 || end < begin || end > a.total) atomicOr(a.err, kErrBadStep);
     }

@@ -1255,7 +1255,9 @@ int step_prompt(Pool* p, const gkv_prompt_desc* r, cudaStream_t st) {
     a.dtype = r->dtype;
     a.scale = r->scale;
     a.err = ws.d_err;
-    cudaError_t e = launch_prompt_simt(a, st);
+    bool ran = false;
+    cudaError_t e = launch_prompt_tc(a, &ran, st);
+    if (e == cudaSuccess && !ran) e = launch_prompt_simt(a, st);
     if (e != cudaSuccess) return cuda_fail(e, "prompt_attention launch");
     ws.built = false;
     p->last_launches += 1;
