@@ -71,7 +71,7 @@ struct StepBuildArgs {
     // the packed step buffer, with every array at the offset of the reservation's maxima
     unsigned char* meta;
     int32_t off_ctx, off_pseg, off_pc0, off_pc1, off_pslot, off_pmerge, off_wbeg, off_mseg, off_ms0, off_mns, off_mdef;
-    int32_t* scratch;                                // 2 * batch * heads_kv ints
+    int32_t* scratch;                                // 3 * batch * heads_kv ints
     int* err;
 };
 cudaError_t launch_step_build(const StepBuildArgs& a, cudaStream_t st);

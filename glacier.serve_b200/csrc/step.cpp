@@ -575,7 +575,7 @@ int step_build(Pool* p, const gkv_step_io* io, int32_t batch, cudaStream_t st) {
     const int64_t workers = static_cast<int64_t>(ws.n_ctas_max) * ws.cfg.warps;
     const int64_t n_seg = static_cast<int64_t>(ws.max_batch) * p->desc.heads_kv;
     const MetaLayout L = meta_layout(ws.max_tokens, ws.max_batch, 0, workers + n_seg, workers, n_seg);
-    if (L.total > ws.meta_cap || static_cast<size_t>(n_seg) * 8 > ws.meta_cap || L.total > 0x7fffffff)
+    if (L.total > ws.meta_cap || static_cast<size_t>(n_seg) * 12 > ws.meta_cap || L.total > 0x7fffffff)
         return set_error(GKV_ESTATE, "static step buffer too small");
     StepBuildArgs a{};
     a.ctx_lens = io->d_ctx_lens;

@@ -275,7 +275,8 @@ typedef struct gkv_step_io {
  * until they have run.  A request is left out of the step (slots -1, decode output untouched, table
  * and ctx_out as before, GKV_EDEVICE from the next gkv_sync) when a length is negative, c + n
  * exceeds table_stride * block_size, its pages need more than n_new_blocks ids or its rows more
- * than max_tokens.  A block id outside the pool gives slot -1 and GKV_EDEVICE.  batch is at most
+ * than max_tokens; all of them are left out of the decode (alone) when heads_kv times the chunks of 8
+ * tokens they attend, plus 4 each, reach 2^31.  A block id outside the pool gives slot -1 and GKV_EDEVICE.  batch is at most
  * the reservation's and 4096, max_tokens at most the reservation's; d_ctx_out must not overlap
  * d_ctx_lens or d_new_lens.  No reference counterpart (the reference packs tables on the host,
  * CudaPagedTransformerRunner.cs:367-379). */

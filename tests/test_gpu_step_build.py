@@ -191,14 +191,14 @@ def test_refusals(cuda):
 
 
 @pytest.mark.parametrize("dtype,heads,heads_kv,dim", [("f32", 28, 4, 128), ("bf16", 28, 4, 128), ("fp8", 28, 4, 128), ("bf16", 8, 8, 64)])
-@pytest.mark.parametrize("kind", ["one long", "mixed", "many short", "few units"])
+@pytest.mark.parametrize("kind", ["one long", "mixed", "many short", "few units", "fewer units than workers"])
 def test_decode_on_the_built_step(cuda, dtype, heads, heads_kv, dim, kind):
     """The decode right behind the build, and behind an append, equals the uploaded step's bit for bit."""
     import torch
 
     rng = np.random.default_rng(heads + len(kind))
     ctx = {"one long": [20000], "mixed": [3, 0, 777, 4000, 16, 1, 0, 12000], "many short": rng.integers(0, 40, 300).tolist(),
-           "few units": [1, 0, 2, 1]}[kind]
+           "few units": [1, 0, 2, 1], "fewer units than workers": [71, 1, 0, 301, 17, 0, 0, 40]}[kind]
     new = [1 if i % 3 != 1 else 0 for i in range(len(ctx))]
     tables, ids, total = _case(rng, ctx, new, 16)
     pool = G.PagedBlockPool(total, 1, heads_kv, dim, 16, dtype=dtype)
@@ -230,4 +230,30 @@ def test_decode_on_the_built_step(cuda, dtype, heads, heads_kv, dim, kind):
     assert torch.equal(outs[2][0], outs[3][0])
     idle = torch.tensor([c == 0 for c in want[6]], device="cuda")
     assert bool((outs[1][0][idle] == 3.0).all())
+    pool.close()
+
+
+def test_more_context_than_the_work_list_counts(cuda):
+    """2^31 units and more: slots are built, nothing is decoded, and it is reported."""
+    import torch
+
+    pool = G.PagedBlockPool(1, 1, 32, 32, 1024, dtype="bf16")
+    B, ctx, width = 40, 16_000_000, 15626
+    pool.reserve_step(B, 1, B, 32)
+    pool.set_static_step()
+    t = lambda n: torch.full((B,), n, dtype=torch.int32, device="cuda")  # noqa: E731
+    io = G.StepBuffers(torch.zeros(B, width, dtype=torch.int32, device="cuda"), t(ctx), t(1), t(0), max_tokens=B)  # every request opens a page
+    pool.build_step(io)
+    with pytest.raises(G.DeviceError):
+        pool.sync()
+    assert io.positions.tolist() == [ctx] * B and io.slots.tolist() == [ctx % 1024] * B and io.ctx_out.tolist() == [ctx + 1] * B
+    out = torch.full((B, 32, 32), 3.0, device="cuda")
+    pool.paged_decode(0, torch.zeros_like(out), out, 32, 1.0)
+    pool.sync()
+    assert bool((out == 3.0).all())
+    io.ctx_lens.fill_(5)  # the next step is as any other
+    pool.build_step(io)
+    pool.paged_decode(0, torch.zeros_like(out), out, 32, 1.0)
+    pool.sync()
+    assert bool((out == 0.0).all())
     pool.close()
