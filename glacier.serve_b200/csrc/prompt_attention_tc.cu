@@ -14,12 +14,15 @@
 //    memory, causal mask on the last key tile, online softmax with lazy rescaling (O is rescaled
 //    only where the running maximum grows by more than 2^8, so p stays below 2^8), P back into tensor
 //    memory; at the end O / l through shared memory to whole rows of the output.
-//  * warp 8: one thread issues every product.  S of key tile j + 1 overwrites P of tile j, so it is
-//    issued behind P V of tile j (products of one thread execute in issue order), and a warpgroup
-//    that sees S of tile j + 1 knows that O holds P V of tile j: rescaling needs no further barrier.
-//  * warp 9: one thread loads Q, and K and V tiles in turn through a ring of 4 slots (TMA, 128-byte
+//  * warps 8 and 9, one per query tile: one thread of each issues the tile's products (one thread for
+//    both spent a third of its time on waits and commits with the tensor pipe idle), in turns, so that
+//    the two tiles' softmaxes do not fall together.  S of key tile
+//    j + 1 overwrites P of tile j, so it is issued behind P V of tile j (products of one thread execute
+//    in issue order), and a warpgroup that sees S of tile j + 1 knows that O holds P V of tile j:
+//    rescaling needs no further barrier.
+//  * warp 10: one thread loads Q, and K and V tiles in turn through a ring of 4 slots (TMA, 128-byte
 //    swizzle, no multicast).
-//  * warp 10: finds the next item while the block works on this one.  The grid holds every item, the
+//  * warp 11: finds the next item while the block works on this one.  The grid holds every item, the
 //    longest of a prompt first; a running block takes over blocks that have not started
 //    (clusterlaunchcontrol), so the next item's loads and first scores overlap this one's end.
 // Values that no row may see (keys behind a prompt's end, and not-finite values of keys that some rows
@@ -42,7 +45,7 @@ namespace {
 
 constexpr int kBM = 128, kBN = 128;               // query rows of a tile, keys of a tile
 constexpr int kRows = 2 * kBM;                    // query rows of an item
-constexpr int kMmaWarp = 8, kLoadWarp = 9, kPlanWarp = 10;
+constexpr int kMmaWarp = 8, kLoadWarp = 10, kPlanWarp = 11;  // kMmaWarp + t issues query tile t's products
 constexpr int kThreads = 384;
 constexpr int kRing = 4;
 constexpr uint32_t kTmemCols = 512;               // S0 S1 O0 O1, 128 columns each
@@ -71,9 +74,9 @@ struct Item {
 struct Book {
     uint64_t q_full, q_empty;
     uint64_t ring_full[kRing], ring_empty[kRing];
-    uint64_t s_full[2], p_full[2], o_full[2];
+    uint64_t s_full[2], p_full[2][2], o_full[2];  // p_full: of 64 keys each
     uint64_t item_full, item_empty;
-    uint64_t steal, drained;
+    uint64_t steal, drained[2], turn[2];
     alignas(16) uint32_t response[4];
     Item item;
     uint32_t tmem;
@@ -133,6 +136,28 @@ __device__ __forceinline__ int stolen_block(const uint32_t* response) {
         : "r"(smem_u32(response))
         : "memory");
     return ok ? static_cast<int>(x) : -1;
+}
+
+// Of every 4 pairs of a row, those whose exponential runs on the FMA pipe.
+constexpr int kFmaPairs = 0;
+
+// 2^x of two values on the FMA pipe: x = n + f with n the nearest whole number and |f| <= 1/2, 2^f by a
+// polynomial of degree 4 (fitted to the least largest relative error, 2.6e-6), n added to the exponent.
+// x at most 127; below -126 the result is 0 (2^-126 is taken off, which no other result notices).
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+    constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it leaves n in the low bits
+    x = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+    const float2 r = __fadd2_rn(x, make_float2(kRound, kRound));
+    const float2 n = __fadd2_rn(r, make_float2(-kRound, -kRound));
+    const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+    float2 p = make_float2(0.00957004725933075f, 0.00957004725933075f);
+    p = __ffma2_rn(p, f, make_float2(0.05591774731874466f, 0.05591774731874466f));
+    p = __ffma2_rn(p, f, make_float2(0.240247443318367f, 0.240247443318367f));
+    p = __ffma2_rn(p, f, make_float2(0.6931218504905701f, 0.6931218504905701f));
+    p = __ffma2_rn(p, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
+    p.x = __uint_as_float(__float_as_uint(p.x) + (__float_as_uint(r.x) << 23));
+    p.y = __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(r.y) << 23));
+    return __fadd2_rn(p, make_float2(-0x1p-126f, -0x1p-126f));
 }
 
 template <bool F16>
@@ -200,21 +225,23 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (threadIdx.x == 0) {
         mbar_init(&bk->q_full, 1);
-        mbar_init(&bk->q_empty, 1);
+        mbar_init(&bk->q_empty, 2);
         for (int i = 0; i < kRing; ++i) {
             mbar_init(&bk->ring_full[i], 1);
-            mbar_init(&bk->ring_empty[i], 1);
+            mbar_init(&bk->ring_empty[i], 2);
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(&bk->s_full[t], 1);
-            mbar_init(&bk->p_full[t], 128);
+            mbar_init(&bk->p_full[t][0], 128);
+            mbar_init(&bk->p_full[t][1], 128);
+            mbar_init(&bk->drained[t], 1);
+            mbar_init(&bk->turn[t], 1);
             mbar_init(&bk->o_full[t], 1);
             bk->poisoned[t][0] = bk->poisoned[t][1] = 0;
         }
         mbar_init(&bk->item_full, 1);
-        mbar_init(&bk->item_empty, 10);  // both warpgroups' warps, the issuer, the loader
+        mbar_init(&bk->item_empty, 11);  // both warpgroups' warps, the issuers, the loader
         mbar_init(&bk->steal, 1);
-        mbar_init(&bk->drained, 1);
         bk->abort = 0;
         fence_mbar_init();
     }
@@ -226,6 +253,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = bk->tmem;
     bool ok = true;
 
+    // registers: 384 x 168 at launch = 128 x (208 + 208 + 88)
+    if (warp >= 8) {
+    fewer_registers<88>();
     if (warp == kPlanWarp) {
         // ---------------- items ----------------
         if (blockIdx.x == 0) check_prompts(a, lane, 32);
@@ -307,19 +337,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (uint32_t s = slot > kRing ? slot - kRing : 0; s < slot; ++s) mbar_wait(&bk->ring_full[s % kRing], (s / kRing) & 1);
             }
         }
-    } else if (warp == kMmaWarp) {
-        // ---------------- products ----------------
+    } else {
+        // ---------------- products of query tile t ----------------
         if (lane == 0) {
             constexpr uint32_t kIdS = idesc_16(kBM, kBN, false, F16);
             constexpr uint32_t kIdO = idesc_16(kBM, D, true, F16);
+            const int t = warp - kMmaWarp;
+            const uint32_t tS = tmem + kColS + t * 128, tO = tmem + kColO + t * 128;
+            // descriptors' low words advance by bytes / 16
+            const uint64_t q_desc = umma_desc_sw128(smem_u32(sQ) + t * Sh::kTile, 16, 1024);
+            const uint64_t k_desc = umma_desc_sw128(smem_u32(sRing), 16, 1024);
+            const uint64_t v_desc = umma_desc_sw128(smem_u32(sRing), Sh::kHalf, 1024);
             uint32_t slot = 0;          // ring position of the next tile
-            uint32_t p_count[2] = {0, 0};
-            auto scores = [&](int t, uint32_t ks) {  // S_t = Q_t K^T
-                const uint32_t q = smem_u32(sQ) + t * Sh::kTile, k = smem_u32(sRing) + ks * Sh::kTile;
+            uint32_t p_count = 0, turns = 0;
+            auto full = [&](uint32_t at) { return wait(&bk->ring_full[at % kRing], (at / kRing) & 1, bk); };
+            auto scores = [&](uint32_t at) {  // S = Q K^T
+                const uint64_t k = k_desc + (at % kRing) * (Sh::kTile / 16);
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk)
-                    umma_f16(tmem + kColS + t * 128, umma_desc_sw128(q + (kk >> 2) * Sh::kHalf + (kk & 3) * 32, 16, 1024),
-                             umma_desc_sw128(k + (kk >> 2) * Sh::kHalf + (kk & 3) * 32, 16, 1024), kIdS, kk > 0 ? 1u : 0u);
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    const uint32_t off = ((kk >> 2) * Sh::kHalf + (kk & 3) * 32) / 16;
+                    umma_f16(tS, q_desc + off, k + off, kIdS, kk > 0 ? 1u : 0u);
+                }
                 umma_commit(&bk->s_full[t]);
             };
             for (uint32_t i = 0;; ++i) {
@@ -327,57 +365,68 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int n0 = bk->item.n[0], n1 = bk->item.n[1];
                 mbar_arrive(&bk->item_empty);
                 if (n0 == 0) break;
-                const int n[2] = {n0, n1};
-                const int nj = n1 ? n1 : n0;
-                uint32_t ks = slot % kRing;
-                if (!(ok = wait(&bk->ring_full[ks], (slot / kRing) & 1, bk) && wait(&bk->q_full, i & 1, bk))) break;
+                const int n = t ? n1 : n0, nj = n1 ? n1 : n0;
+                // a slot is free when both tiles are done with it: behind this tile's products so far, or,
+                // where it has none, as soon as the slot is filled
+                if (!(ok = wait(&bk->q_full, i & 1, bk) && full(slot))) break;
                 tc_fence_after();
-                scores(0, ks);
-                if (n1) scores(1, ks);
-                umma_commit(&bk->ring_empty[ks]);
-                if (nj == 1) umma_commit(&bk->q_empty);
-                ++slot;
-                for (int j = 0; ok && j < nj; ++j) {
-                    const uint32_t vs = slot % kRing;
-                    if (!(ok = wait(&bk->ring_full[vs], (slot / kRing) & 1, bk))) break;
-                    ++slot;
+                if (n > 0) {
+                    scores(slot);
+                    umma_commit(&bk->ring_empty[slot % kRing]);
+                    if (n == 1) umma_commit(&bk->q_empty);
+                } else {
+                    mbar_arrive(&bk->ring_empty[slot % kRing]);
+                    mbar_arrive(&bk->q_empty);
+                }
+                for (int j = 0; j < nj; ++j) {
+                    const uint32_t vs = slot + 2 * j + 1, ks = vs + 1;  // V of tile j, K of tile j + 1
                     const bool more = j + 1 < nj;
-                    ks = slot % kRing;
-                    if (more && !(ok = wait(&bk->ring_full[ks], (slot / kRing) & 1, bk))) break;
-                    slot += more ? 1 : 0;
+                    if (!(ok = full(vs) && (!more || full(ks)))) break;
+                    // the tiles' products go in turns, the first tile's of every key tile first
+                    const uint32_t mine = (turns + (t ^ 1)) & 1;
+                    ++turns;
+                    if (j >= n) {
+                        mbar_arrive(&bk->ring_empty[vs % kRing]);
+                        if (more) mbar_arrive(&bk->ring_empty[ks % kRing]);
+                        if (!(ok = wait(&bk->turn[t], mine, bk))) break;
+                        mbar_arrive(&bk->turn[t ^ 1]);
+                        continue;
+                    }
+                    const uint64_t v = v_desc + (vs % kRing) * (Sh::kTile / 16);
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        if (j >= n[t]) continue;
-                        if (!(ok = wait(&bk->p_full[t], p_count[t] & 1, bk))) break;
-                        ++p_count[t];
+                    for (int half = 0; half < 2; ++half) {
+                        if (!(ok = wait(&bk->p_full[t][half], p_count & 1, bk) && (half || wait(&bk->turn[t], mine, bk)))) break;
                         tc_fence_after();
-                        const uint32_t v = smem_u32(sRing) + vs * Sh::kTile;
 #pragma unroll
-                        for (int kk = 0; kk < kBN / 16; ++kk)
+                        for (int k4 = 0; k4 < kBN / 32; ++k4) {
+                            const int kk = half * (kBN / 32) + k4;
                             // V tile [key][dim]: MN-major, 8-key groups 1 KB apart, dims 64-127 in the second half
-                            umma_f16_ts(tmem + kColO + t * 128, tmem + kColS + t * 128 + kk * 8,
-                                        umma_desc_sw128(v + kk * 2048, Sh::kHalf, 1024), kIdO, (j > 0 || kk > 0) ? 1u : 0u);
-                        if (j + 1 < n[t]) scores(t, ks);
-                        else umma_commit(&bk->o_full[t]);
+                            umma_f16_ts(tO, tS + kk * 8, v + kk * (2048 / 16), kIdO, (j > 0 || kk > 0) ? 1u : 0u);
+                        }
                     }
                     if (!ok) break;
-                    umma_commit(&bk->ring_empty[vs]);
-                    if (more) {
-                        umma_commit(&bk->ring_empty[ks]);
-                        if (j + 2 == nj) umma_commit(&bk->q_empty);
-                    }
+                    ++p_count;
+                    if (j + 1 < n) scores(ks);
+                    else umma_commit(&bk->o_full[t]);
+                    mbar_arrive(&bk->turn[t ^ 1]);
+                    umma_commit(&bk->ring_empty[vs % kRing]);
+                    if (more) umma_commit(&bk->ring_empty[ks % kRing]);
+                    if (j + 2 == n) umma_commit(&bk->q_empty);
                 }
                 if (!ok) break;
+                slot += 2 * nj;
             }
             if (!ok) {
                 bk->abort = 1;
                 atomicOr(a.err, kErrWaitTimeout);
             }
-            umma_commit(&bk->drained);  // every product is complete before the tensor memory is freed
-            if (!mbar_wait(&bk->drained, 0)) atomicOr(a.err, kErrWaitTimeout);
+            umma_commit(&bk->drained[t]);  // every product is complete before the tensor memory is freed
+            if (!mbar_wait(&bk->drained[t], 0)) atomicOr(a.err, kErrWaitTimeout);
         }
-    } else if (warp < 8) {
+    }
+    } else {
         // ---------------- softmax and epilogue ----------------
+        more_registers<208>();
         const int t = warp >> 2, r = threadIdx.x & 127;
         const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
         const uint32_t tS = tmem + kColS + t * 128 + lanes, tO = tmem + kColO + t * 128 + lanes;
@@ -437,31 +486,37 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tmem_st32(tO + c * 32, o);
                     }
                 }
-                const float2 sl2 = make_float2(sl, sl), nm2 = make_float2(-m_run, -m_run);
-                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t pk[32];
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const uint32_t* x = &s[2 * c + (e >> 4)][(e & 15) * 2];
-                        const float2 y = __ffma2_rn(make_float2(__uint_as_float(x[0]), __uint_as_float(x[1])), sl2, nm2);
-                        const float2 p = make_float2(fast_exp2(y.x), fast_exp2(y.y));
-                        sum[e & 1] = __fadd2_rn(sum[e & 1], p);
-                        pk[e] = pack_16x2<F16>(p.x, p.y);
-                    }
-                    tmem_st32(tS + c * 32, pk);  // P over the first 64 columns of S
-                }
-                l_run += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 if (j == n - 1) {
                     const uint32_t vs = slot0 + 2 * j + 1;
                     if (!(ok = __all_sync(~0u, wait(&bk->ring_full[vs % kRing], (vs / kRing) & 1, bk)))) break;
                     clean_values<D, F16>(sRing + (vs % kRing) * Sh::kTile, r, j * kBN + r, it.len, bk, it.number, t);
                     fence_proxy_async_smem();
                 }
+                // p of 32 keys at a time into the first 64 columns of S; the products of the first 64 keys may
+                // start while the others are on their way
+                const float2 sl2 = make_float2(sl, sl), nm2 = make_float2(-m_run, -m_run);
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float2 y = __ffma2_rn(make_float2(__uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1])), sl2, nm2);
+                        const float2 p = (e & 3) < kFmaPairs ? exp2_fma(y) : make_float2(fast_exp2(y.x), fast_exp2(y.y));
+                        sum[e & 1] = __fadd2_rn(sum[e & 1], p);
+                        pk[e] = pack_16x2<F16>(p.x, p.y);
+                    }
+                    if (c == 2) {
+                        tmem_wait_st();
+                        tc_fence_before();
+                        mbar_arrive(&bk->p_full[t][0]);
+                    }
+                    tmem_st16(tS + c * 16, pk);
+                }
+                l_run += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(&bk->p_full[t]);
+                mbar_arrive(&bk->p_full[t][1]);
             }
             slot0 += 2 * nj;
             if (!ok || n == 0) continue;
