@@ -304,6 +304,17 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
         : "memory");
 }
 
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_lane() {
+    uint32_t mine;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(mine));
+    return mine != 0;
+}
+
 // Moves registers between the warpgroups of a block: every warp of a warpgroup executes one of these.
 // The shares of all warpgroups must fit what the block was launched with (threads x registers each).
 template <int N>

@@ -52,6 +52,8 @@ constexpr uint32_t kTmemCols = 512;               // S0 S1 O0 O1, 128 columns ea
 constexpr uint32_t kColS = 0, kColO = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleLog2 = 8.f;
+constexpr uint32_t kPolls = 1u << 24;
+constexpr uint32_t kPlanNs = 1000, kLoadNs = 200, kMmaNs = 0, kSoftNs = 0;
 
 template <int D>
 struct Shape {
@@ -96,10 +98,12 @@ constexpr uint32_t idesc_16(int m, int n, bool b_mn_major, bool f16) {
            (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-// Bounded wait that also ends (false) when the block has given up.
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Book* bk) {
+// Bounded wait that also ends (false) when the block has given up.  Between polls the thread sleeps
+// for about `ns` nanoseconds: polls take the issue slots and the queue of the exponentials that the
+// other warps need.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Book* bk, uint32_t ns) {
     const uint32_t addr = smem_u32(bar);
-    for (uint32_t it = 0; it < kWaitLimit; ++it) {
+    for (uint32_t it = 0; it < kPolls; ++it) {
         uint32_t done;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
@@ -109,7 +113,8 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Book* bk) {
             : "r"(addr), "r"(parity)
             : "memory");
         if (done) return true;
-        if ((it & 63) == 63 && *reinterpret_cast<volatile int*>(&bk->abort)) return false;
+        if ((it & 15) == 15 && *reinterpret_cast<volatile int*>(&bk->abort)) return false;
+        if (ns) __nanosleep(ns);
     }
     return false;
 }
@@ -284,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 if (block < 0) break;
                 // the next item is fetched once every warp has begun this one
-                if (!(ok = __all_sync(~0u, wait(&bk->item_empty, published & 1, bk)))) break;
+                if (!(ok = __all_sync(~0u, wait(&bk->item_empty, published & 1, bk, kPlanNs)))) break;
                 ++published;
             }
             if (lane == 0) steal_block(bk->response, &bk->steal);
@@ -304,11 +309,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) {
             uint32_t slot = 0, q_loads = 0;
             for (uint32_t i = 0;; ++i) {
-                if (!(ok = wait(&bk->item_full, i & 1, bk))) break;
+                if (!(ok = wait(&bk->item_full, i & 1, bk, kLoadNs))) break;
                 const Item it = bk->item;
                 mbar_arrive(&bk->item_empty);
                 if (it.n[0] == 0) break;
-                if (i > 0 && !(ok = wait(&bk->q_empty, (i - 1) & 1, bk))) break;
+                if (i > 0 && !(ok = wait(&bk->q_empty, (i - 1) & 1, bk, kLoadNs))) break;
                 const int kv = it.head / (a.n_heads / a.heads_kv);
                 const int row = static_cast<int>(it.row0) + it.q0;
                 mbar_arrive_expect_tx(&bk->q_full, it.n[1] ? 2 * Sh::kTile : Sh::kTile);
@@ -321,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 load(sQ, &tmq, it.head, row, &bk->q_full);
                 for (int j = 0; j < 2 * nj; ++j) {  // K of tile j / 2, then V
                     const int s = slot % kRing;
-                    if (slot >= kRing && !(ok = wait(&bk->ring_empty[s], (slot / kRing - 1) & 1, bk))) break;
+                    if (slot >= kRing && !(ok = wait(&bk->ring_empty[s], (slot / kRing - 1) & 1, bk, kLoadNs))) break;
                     mbar_arrive_expect_tx(&bk->ring_full[s], Sh::kTile);
                     load(sRing + s * Sh::kTile, (j & 1) ? &tmv : &tmk, kv, static_cast<int>(it.row0) + (j >> 1) * kBN, &bk->ring_full[s]);
                     ++slot;
@@ -339,37 +344,43 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else {
         // ---------------- products of query tile t ----------------
-        if (lane == 0) {
-            constexpr uint32_t kIdS = idesc_16(kBM, kBN, false, F16);
-            constexpr uint32_t kIdO = idesc_16(kBM, D, true, F16);
-            const int t = warp - kMmaWarp;
-            const uint32_t tS = tmem + kColS + t * 128, tO = tmem + kColO + t * 128;
-            // descriptors' low words advance by bytes / 16
-            const uint64_t q_desc = umma_desc_sw128(smem_u32(sQ) + t * Sh::kTile, 16, 1024);
-            const uint64_t k_desc = umma_desc_sw128(smem_u32(sRing), 16, 1024);
-            const uint64_t v_desc = umma_desc_sw128(smem_u32(sRing), Sh::kHalf, 1024);
-            uint32_t slot = 0;          // ring position of the next tile
-            uint32_t p_count = 0, turns = 0;
-            auto full = [&](uint32_t at) { return wait(&bk->ring_full[at % kRing], (at / kRing) & 1, bk); };
-            auto scores = [&](uint32_t at) {  // S = Q K^T
-                const uint64_t k = k_desc + (at % kRing) * (Sh::kTile / 16);
+        // The whole warp keeps the loop, so that ring positions and descriptors are the same for all its
+        // lanes (in uniform registers, where the products take them); one lane issues.
+        constexpr uint32_t kIdS = idesc_16(kBM, kBN, false, F16);
+        constexpr uint32_t kIdO = idesc_16(kBM, D, true, F16);
+        const int t = __shfl_sync(~0u, warp, 0) - kMmaWarp;
+        const uint32_t tm = __shfl_sync(~0u, tmem, 0);
+        const uint32_t tS = tm + kColS + t * 128, tO = tm + kColO + t * 128;
+        const bool issuer = elect_lane();
+        // descriptors' low words advance by bytes / 16
+        const uint64_t q_desc = umma_desc_sw128(smem_u32(sQ) + t * Sh::kTile, 16, 1024);
+        const uint64_t k_desc = umma_desc_sw128(smem_u32(sRing), 16, 1024);
+        const uint64_t v_desc = umma_desc_sw128(smem_u32(sRing), Sh::kHalf, 1024);
+        uint32_t slot = 0;          // ring position of the next tile
+        uint32_t p_count = 0, turns = 0;
+        auto ready = [&](uint64_t* bar, uint32_t parity) { return __all_sync(~0u, wait(bar, parity, bk, kMmaNs)) != 0; };
+        auto full = [&](uint32_t at) { return ready(&bk->ring_full[at % kRing], (at / kRing) & 1); };
+        auto scores = [&](uint32_t at) {  // S = Q K^T
+            const uint64_t k = k_desc + (at % kRing) * (Sh::kTile / 16);
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t off = ((kk >> 2) * Sh::kHalf + (kk & 3) * 32) / 16;
-                    umma_f16(tS, q_desc + off, k + off, kIdS, kk > 0 ? 1u : 0u);
-                }
-                umma_commit(&bk->s_full[t]);
-            };
-            for (uint32_t i = 0;; ++i) {
-                if (!(ok = wait(&bk->item_full, i & 1, bk))) break;
-                const int n0 = bk->item.n[0], n1 = bk->item.n[1];
-                mbar_arrive(&bk->item_empty);
-                if (n0 == 0) break;
-                const int n = t ? n1 : n0, nj = n1 ? n1 : n0;
-                // a slot is free when both tiles are done with it: behind this tile's products so far, or,
-                // where it has none, as soon as the slot is filled
-                if (!(ok = wait(&bk->q_full, i & 1, bk) && full(slot))) break;
-                tc_fence_after();
+            for (int kk = 0; kk < D / 16; ++kk) {
+                const uint32_t off = ((kk >> 2) * Sh::kHalf + (kk & 3) * 32) / 16;
+                umma_f16(tS, q_desc + off, k + off, kIdS, kk > 0 ? 1u : 0u);
+            }
+            umma_commit(&bk->s_full[t]);
+        };
+        for (uint32_t i = 0;; ++i) {
+            if (!(ok = ready(&bk->item_full, i & 1))) break;
+            const int n0 = __shfl_sync(~0u, bk->item.n[0], 0), n1 = __shfl_sync(~0u, bk->item.n[1], 0);
+            __syncwarp();
+            if (issuer) mbar_arrive(&bk->item_empty);
+            if (n0 == 0) break;
+            const int n = t ? n1 : n0, nj = n1 ? n1 : n0;
+            // a slot is free when both tiles are done with it: behind this tile's products so far, or,
+            // where it has none, as soon as the slot is filled
+            if (!(ok = ready(&bk->q_full, i & 1) && full(slot))) break;
+            tc_fence_after();
+            if (issuer) {
                 if (n > 0) {
                     scores(slot);
                     umma_commit(&bk->ring_empty[slot % kRing]);
@@ -378,34 +389,41 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mbar_arrive(&bk->ring_empty[slot % kRing]);
                     mbar_arrive(&bk->q_empty);
                 }
-                for (int j = 0; j < nj; ++j) {
-                    const uint32_t vs = slot + 2 * j + 1, ks = vs + 1;  // V of tile j, K of tile j + 1
-                    const bool more = j + 1 < nj;
-                    if (!(ok = full(vs) && (!more || full(ks)))) break;
-                    // the tiles' products go in turns, the first tile's of every key tile first
-                    const uint32_t mine = (turns + (t ^ 1)) & 1;
-                    ++turns;
-                    if (j >= n) {
+            }
+            __syncwarp();
+            for (int j = 0; j < nj; ++j) {
+                const uint32_t vs = slot + 2 * j + 1, ks = vs + 1;  // V of tile j, K of tile j + 1
+                const bool more = j + 1 < nj;
+                if (!(ok = full(vs) && (!more || full(ks)))) break;
+                // the tiles' products go in turns, the first tile's of every key tile first
+                const uint32_t mine = (turns + (t ^ 1)) & 1;
+                ++turns;
+                if (j < n && !(ok = ready(&bk->p_full[t][0], p_count & 1))) break;
+                if (!(ok = ready(&bk->turn[t], mine))) break;
+                if (j >= n) {
+                    if (issuer) {
                         mbar_arrive(&bk->ring_empty[vs % kRing]);
                         if (more) mbar_arrive(&bk->ring_empty[ks % kRing]);
-                        if (!(ok = wait(&bk->turn[t], mine, bk))) break;
                         mbar_arrive(&bk->turn[t ^ 1]);
-                        continue;
                     }
-                    const uint64_t v = v_desc + (vs % kRing) * (Sh::kTile / 16);
+                    __syncwarp();
+                    continue;
+                }
+                const uint64_t v = v_desc + (vs % kRing) * (Sh::kTile / 16);
+                // V tile [key][dim]: MN-major, 8-key groups 1 KB apart, dims 64-127 in the second half
+                auto values = [&](int kk) { umma_f16_ts(tO, tS + kk * 8, v + kk * (2048 / 16), kIdO, (j > 0 || kk > 0) ? 1u : 0u); };
+                tc_fence_after();
+                if (issuer) {
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        if (!(ok = wait(&bk->p_full[t][half], p_count & 1, bk) && (half || wait(&bk->turn[t], mine, bk)))) break;
-                        tc_fence_after();
+                    for (int kk = 0; kk < kBN / 32; ++kk) values(kk);
+                }
+                __syncwarp();
+                if (!(ok = ready(&bk->p_full[t][1], p_count & 1))) break;
+                tc_fence_after();
+                ++p_count;
+                if (issuer) {
 #pragma unroll
-                        for (int k4 = 0; k4 < kBN / 32; ++k4) {
-                            const int kk = half * (kBN / 32) + k4;
-                            // V tile [key][dim]: MN-major, 8-key groups 1 KB apart, dims 64-127 in the second half
-                            umma_f16_ts(tO, tS + kk * 8, v + kk * (2048 / 16), kIdO, (j > 0 || kk > 0) ? 1u : 0u);
-                        }
-                    }
-                    if (!ok) break;
-                    ++p_count;
+                    for (int kk = kBN / 32; kk < kBN / 16; ++kk) values(kk);
                     if (j + 1 < n) scores(ks);
                     else umma_commit(&bk->o_full[t]);
                     mbar_arrive(&bk->turn[t ^ 1]);
@@ -413,9 +431,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (more) umma_commit(&bk->ring_empty[ks % kRing]);
                     if (j + 2 == n) umma_commit(&bk->q_empty);
                 }
-                if (!ok) break;
-                slot += 2 * nj;
+                __syncwarp();
             }
+            if (!ok) break;
+            slot += 2 * nj;
+        }
+        if (issuer) {
             if (!ok) {
                 bk->abort = 1;
                 atomicOr(a.err, kErrWaitTimeout);
@@ -434,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t s_count = 0, o_count = 0;
         uint32_t slot0 = 0;  // ring position of the item's first tile
         for (uint32_t i = 0; ok; ++i) {
-            if (!(ok = __all_sync(~0u, wait(&bk->item_full, i & 1, bk)))) break;
+            if (!(ok = __all_sync(~0u, wait(&bk->item_full, i & 1, bk, kSoftNs)))) break;
             const Item it = bk->item;
             __syncwarp();
             if (lane == 0) mbar_arrive(&bk->item_empty);
@@ -444,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int pos = it.q0 + t * kBM + r;
             float m_run = -INFINITY, l_run = 0.f;
             for (int j = 0; j < n; ++j) {
-                if (!(ok = __all_sync(~0u, wait(&bk->s_full[t], s_count & 1, bk)))) break;
+                if (!(ok = __all_sync(~0u, wait(&bk->s_full[t], s_count & 1, bk, kSoftNs)))) break;
                 ++s_count;
                 tc_fence_after();
                 uint32_t s[4][32];
@@ -457,15 +478,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int c = 0; c < 128; ++c)
                         if (c > limit) s[c >> 5][c & 31] = 0xff800000u;
                 }
+                // eight interleaved chains: a warp has one other on its scheduler to hide its latencies
                 float mq[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const uint32_t* x = &s[k >> 1][(k & 1) * 16];
-                    float m = __uint_as_float(x[0]);
+                for (int k = 0; k < 8; ++k) mq[k] = __uint_as_float(s[k >> 1][(k & 1) * 16]);
 #pragma unroll
-                    for (int e = 1; e < 15; e += 2) m = fmax3(m, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-                    mq[k] = fmaxf(m, __uint_as_float(x[15]));
-                }
+                for (int e = 1; e < 15; e += 2)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        mq[k] = fmax3(mq[k], __uint_as_float(s[k >> 1][(k & 1) * 16 + e]), __uint_as_float(s[k >> 1][(k & 1) * 16 + e + 1]));
+#pragma unroll
+                for (int k = 0; k < 8; ++k) mq[k] = fmaxf(mq[k], __uint_as_float(s[k >> 1][(k & 1) * 16 + 15]));
                 const float mt = fmax3(fmax3(mq[0], mq[1], mq[2]), fmax3(mq[3], mq[4], mq[5]), fmaxf(mq[6], mq[7])) * sl;
                 const bool need = mt > m_run + kRescaleLog2;
                 float alpha = 1.f;
@@ -488,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (j == n - 1) {
                     const uint32_t vs = slot0 + 2 * j + 1;
-                    if (!(ok = __all_sync(~0u, wait(&bk->ring_full[vs % kRing], (vs / kRing) & 1, bk)))) break;
+                    if (!(ok = __all_sync(~0u, wait(&bk->ring_full[vs % kRing], (vs / kRing) & 1, bk, kSoftNs)))) break;
                     clean_values<D, F16>(sRing + (vs % kRing) * Sh::kTile, r, j * kBN + r, it.len, bk, it.number, t);
                     fence_proxy_async_smem();
                 }
@@ -520,7 +543,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             slot0 += 2 * nj;
             if (!ok || n == 0) continue;
-            if (!(ok = __all_sync(~0u, wait(&bk->o_full[t], o_count & 1, bk)))) break;
+            if (!(ok = __all_sync(~0u, wait(&bk->o_full[t], o_count & 1, bk, kSoftNs)))) break;
             ++o_count;
             tc_fence_after();
             // the sink joins the sum against the larger of the two maxima
