@@ -45,6 +45,7 @@ namespace {
 
 constexpr int kBM = 128, kBN = 128;               // query rows of a tile, keys of a tile
 constexpr int kRows = 2 * kBM;                    // query rows of an item
+constexpr int kEarly = 64;                        // keys whose P V starts before the others' p are there (96: 3 % slower)
 constexpr int kMmaWarp = 8, kLoadWarp = 10, kPlanWarp = 11;  // kMmaWarp + t issues query tile t's products
 constexpr int kThreads = 384;
 constexpr int kRing = 4;
@@ -76,7 +77,7 @@ struct Item {
 struct Book {
     uint64_t q_full, q_empty;
     uint64_t ring_full[kRing], ring_empty[kRing];
-    uint64_t s_full[2], p_full[2][2], o_full[2];  // p_full: of 64 keys each
+    uint64_t s_full[2], p_full[2][2], o_full[2];  // p_full: of the first kEarly keys, and of the others
     uint64_t item_full, item_empty;
     uint64_t steal, drained[2], turn[2];
     alignas(16) uint32_t response[4];
@@ -98,23 +99,27 @@ constexpr uint32_t idesc_16(int m, int n, bool b_mn_major, bool f16) {
            (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+__device__ __forceinline__ bool poll(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return done != 0;
+}
 // Bounded wait that also ends (false) when the block has given up.  Between polls the thread sleeps
-// for about `ns` nanoseconds: polls take the issue slots and the queue of the exponentials that the
-// other warps need.
+// for about `ns` nanoseconds: polls take issue slots that the other warps need.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Book* bk, uint32_t ns) {
     const uint32_t addr = smem_u32(bar);
+    if (poll(addr, parity)) return true;
+#pragma unroll 1
     for (uint32_t it = 0; it < kPolls; ++it) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done)
-            : "r"(addr), "r"(parity)
-            : "memory");
-        if (done) return true;
-        if ((it & 15) == 15 && *reinterpret_cast<volatile int*>(&bk->abort)) return false;
         if (ns) __nanosleep(ns);
+        if (poll(addr, parity)) return true;
+        if ((it & 15) == 15 && *reinterpret_cast<volatile int*>(&bk->abort)) return false;
     }
     return false;
 }
@@ -141,28 +146,6 @@ __device__ __forceinline__ int stolen_block(const uint32_t* response) {
         : "r"(smem_u32(response))
         : "memory");
     return ok ? static_cast<int>(x) : -1;
-}
-
-// Of every 4 pairs of a row, those whose exponential runs on the FMA pipe.
-constexpr int kFmaPairs = 0;
-
-// 2^x of two values on the FMA pipe: x = n + f with n the nearest whole number and |f| <= 1/2, 2^f by a
-// polynomial of degree 4 (fitted to the least largest relative error, 2.6e-6), n added to the exponent.
-// x at most 127; below -126 the result is 0 (2^-126 is taken off, which no other result notices).
-__device__ __forceinline__ float2 exp2_fma(float2 x) {
-    constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it leaves n in the low bits
-    x = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
-    const float2 r = __fadd2_rn(x, make_float2(kRound, kRound));
-    const float2 n = __fadd2_rn(r, make_float2(-kRound, -kRound));
-    const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
-    float2 p = make_float2(0.00957004725933075f, 0.00957004725933075f);
-    p = __ffma2_rn(p, f, make_float2(0.05591774731874466f, 0.05591774731874466f));
-    p = __ffma2_rn(p, f, make_float2(0.240247443318367f, 0.240247443318367f));
-    p = __ffma2_rn(p, f, make_float2(0.6931218504905701f, 0.6931218504905701f));
-    p = __ffma2_rn(p, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
-    p.x = __uint_as_float(__float_as_uint(p.x) + (__float_as_uint(r.x) << 23));
-    p.y = __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(r.y) << 23));
-    return __fadd2_rn(p, make_float2(-0x1p-126f, -0x1p-126f));
 }
 
 template <bool F16>
@@ -215,6 +198,122 @@ __device__ __forceinline__ void clean_values(uint8_t* tile, int key, int key_pos
     }
 }
 
+// 2^x, kept in program order.
+__device__ __forceinline__ float exp2_in_order(float x) {
+    float y;
+    asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Weights of 32 keys: p = 2^(sl s - m) of s[0 .. 31], in pairs of the inputs' type; `sum` grows by them.
+// In groups of 8 pairs, the exponentials of a group one after the other and their sums behind them: left
+// to itself the compiler put each sum next to its exponential, and a warp has only one other on its
+// scheduler to fill that wait.
+template <bool F16>
+__device__ __forceinline__ void weights(const uint32_t (&s)[32], float sl, float m, float2 (&sum)[2], uint32_t (&pk)[16]) {
+    const float2 sl2 = make_float2(sl, sl), nm2 = make_float2(-m, -m);
+#pragma unroll
+    for (int g = 0; g < 16; g += 8) {
+        float2 y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            y[e] = __ffma2_rn(make_float2(__uint_as_float(s[2 * (g + e)]), __uint_as_float(s[2 * (g + e) + 1])), sl2, nm2);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = make_float2(exp2_in_order(y[e].x), exp2_in_order(y[e].y));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            sum[e & 1] = __fadd2_rn(sum[e & 1], y[e]);
+            pk[g + e] = pack_16x2<F16>(y[e].x, y[e].y);
+        }
+    }
+}
+__device__ __forceinline__ float largest(const uint32_t (&s)[4][32]) {
+    float mq[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) mq[k] = __uint_as_float(s[k >> 1][(k & 1) * 16]);
+#pragma unroll
+    for (int e = 1; e < 15; e += 2)
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            mq[k] = fmax3(mq[k], __uint_as_float(s[k >> 1][(k & 1) * 16 + e]), __uint_as_float(s[k >> 1][(k & 1) * 16 + e + 1]));
+#pragma unroll
+    for (int k = 0; k < 8; ++k) mq[k] = fmaxf(mq[k], __uint_as_float(s[k >> 1][(k & 1) * 16 + 15]));
+    return fmax3(fmax3(mq[0], mq[1], mq[2]), fmax3(mq[3], mq[4], mq[5]), fmaxf(mq[6], mq[7]));
+}
+__device__ __forceinline__ void p_ready(uint64_t* bar) {
+    tmem_wait_st();
+    tc_fence_before();
+    mbar_arrive(bar);
+}
+
+// The softmax of one key tile, one row per thread: p of 32 keys at a time over the first 64 columns of S.
+// Here with the running maximum m as it was, next to the search for the tile's own; false, with nothing
+// stored, where that is larger by more than 2^8 for some row of the warp.  Straight code: with the mask,
+// the first tile or the rescaling in its blocks the compiler's order cost a long prompt 10 %.
+template <bool F16>
+__device__ __forceinline__ bool middle_tile(uint32_t tS, float sl, float m, float& l, uint64_t* p_full) {
+    uint32_t s[4][32], pk[4][16];
+    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, s[c]);
+    tmem_wait_ld();
+#pragma unroll
+    for (int c = 0; c < kEarly / 32; ++c) weights<F16>(s[c], sl, m, sum, pk[c]);
+    if (__any_sync(~0u, largest(s) * sl > m + kRescaleLog2)) return false;
+#pragma unroll
+    for (int c = 0; c < kEarly / 32; ++c) tmem_st16(tS + c * 16, pk[c]);
+    p_ready(p_full);
+#pragma unroll
+    for (int c = kEarly / 32; c < 4; ++c) {
+        weights<F16>(s[c], sl, m, sum, pk[c]);
+        tmem_st16(tS + c * 16, pk[c]);
+    }
+    p_ready(p_full + 1);
+    l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+    return true;
+}
+
+// The same for any tile: keys behind `limit` masked, the tile's maximum first, O (which holds P V up to
+// the tile before: its products were issued before S of this one) rescaled where it moves the running one.
+template <int D, bool F16>
+__device__ __forceinline__ void any_tile(uint32_t tS, uint32_t tO, float sl, int limit, bool has_o, float& m, float& l, uint64_t* p_full) {
+    uint32_t s[4][32];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, s[c]);
+    tmem_wait_ld();
+#pragma unroll
+    for (int c = 0; c < 128; ++c)
+        if (c > limit) s[c >> 5][c & 31] = 0xff800000u;
+    const float mt = largest(s) * sl;
+    const bool need = mt > m + kRescaleLog2;
+    float alpha = 1.f;
+    if (need) {
+        alpha = fast_exp2(m - mt);  // 0 on the first tile
+        m = mt;
+        l *= alpha;
+    }
+    if (has_o && __any_sync(~0u, need)) {
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(tO + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st32(tO + c * 32, o);
+        }
+    }
+    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        uint32_t pk[16];
+        weights<F16>(s[c], sl, m, sum, pk);
+        tmem_st16(tS + c * 16, pk);
+        if (c == kEarly / 32 - 1) p_ready(p_full);
+    }
+    p_ready(p_full + 1);
+    l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+}
+
 template <int D, bool F16>
 __global__ void __launch_bounds__(kThreads, 1)
     prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
@@ -258,9 +357,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = bk->tmem;
     bool ok = true;
 
-    // registers: 384 x 168 at launch = 128 x (208 + 208 + 88)
+    // registers: 384 x 168 at launch = 128 x (224 + 224 + 56)
     if (warp >= 8) {
-    fewer_registers<88>();
+    fewer_registers<56>();
     if (warp == kPlanWarp) {
         // ---------------- items ----------------
         if (blockIdx.x == 0) check_prompts(a, lane, 32);
@@ -398,7 +497,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // the tiles' products go in turns, the first tile's of every key tile first
                 const uint32_t mine = (turns + (t ^ 1)) & 1;
                 ++turns;
-                if (j < n && !(ok = ready(&bk->p_full[t][0], p_count & 1))) break;
                 if (!(ok = ready(&bk->turn[t], mine))) break;
                 if (j >= n) {
                     if (issuer) {
@@ -410,12 +508,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     continue;
                 }
                 const uint64_t v = v_desc + (vs % kRing) * (Sh::kTile / 16);
+                if (!(ok = ready(&bk->p_full[t][0], p_count & 1))) break;
                 // V tile [key][dim]: MN-major, 8-key groups 1 KB apart, dims 64-127 in the second half
                 auto values = [&](int kk) { umma_f16_ts(tO, tS + kk * 8, v + kk * (2048 / 16), kIdO, (j > 0 || kk > 0) ? 1u : 0u); };
                 tc_fence_after();
                 if (issuer) {
 #pragma unroll
-                    for (int kk = 0; kk < kBN / 32; ++kk) values(kk);
+                    for (int kk = 0; kk < kEarly / 16; ++kk) values(kk);
                 }
                 __syncwarp();
                 if (!(ok = ready(&bk->p_full[t][1], p_count & 1))) break;
@@ -423,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ++p_count;
                 if (issuer) {
 #pragma unroll
-                    for (int kk = kBN / 32; kk < kBN / 16; ++kk) values(kk);
+                    for (int kk = kEarly / 16; kk < kBN / 16; ++kk) values(kk);
                     if (j + 1 < n) scores(ks);
                     else umma_commit(&bk->o_full[t]);
                     mbar_arrive(&bk->turn[t ^ 1]);
@@ -447,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     } else {
         // ---------------- softmax and epilogue ----------------
-        more_registers<208>();
+        more_registers<224>();
         const int t = warp >> 2, r = threadIdx.x & 127;
         const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
         const uint32_t tS = tmem + kColS + t * 128 + lanes, tO = tmem + kColO + t * 128 + lanes;
@@ -468,78 +567,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!(ok = __all_sync(~0u, wait(&bk->s_full[t], s_count & 1, bk, kSoftNs)))) break;
                 ++s_count;
                 tc_fence_after();
-                uint32_t s[4][32];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, s[c]);
-                tmem_wait_ld();
-                if (j == n - 1) {
-                    const int limit = pos - j * kBN;  // keys 0 .. limit of the tile
-#pragma unroll
-                    for (int c = 0; c < 128; ++c)
-                        if (c > limit) s[c >> 5][c & 31] = 0xff800000u;
-                }
-                // eight interleaved chains: a warp has one other on its scheduler to hide its latencies
-                float mq[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) mq[k] = __uint_as_float(s[k >> 1][(k & 1) * 16]);
-#pragma unroll
-                for (int e = 1; e < 15; e += 2)
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        mq[k] = fmax3(mq[k], __uint_as_float(s[k >> 1][(k & 1) * 16 + e]), __uint_as_float(s[k >> 1][(k & 1) * 16 + e + 1]));
-#pragma unroll
-                for (int k = 0; k < 8; ++k) mq[k] = fmaxf(mq[k], __uint_as_float(s[k >> 1][(k & 1) * 16 + 15]));
-                const float mt = fmax3(fmax3(mq[0], mq[1], mq[2]), fmax3(mq[3], mq[4], mq[5]), fmaxf(mq[6], mq[7])) * sl;
-                const bool need = mt > m_run + kRescaleLog2;
-                float alpha = 1.f;
-                if (need) {
-                    alpha = fast_exp2(m_run - mt);  // 0 on the first tile
-                    m_run = mt;
-                    l_run *= alpha;
-                }
-                if (j > 0 && __any_sync(~0u, need)) {
-                    // O holds P V up to tile j - 1: its products were issued before S of this tile
-#pragma unroll 1
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t o[32];
-                        tmem_ld32(tO + c * 32, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                        tmem_st32(tO + c * 32, o);
-                    }
-                }
+                if (j > 0 && j < n - 1 && middle_tile<F16>(tS, sl, m_run, l_run, bk->p_full[t])) continue;
                 if (j == n - 1) {
                     const uint32_t vs = slot0 + 2 * j + 1;
                     if (!(ok = __all_sync(~0u, wait(&bk->ring_full[vs % kRing], (vs / kRing) & 1, bk, kSoftNs)))) break;
                     clean_values<D, F16>(sRing + (vs % kRing) * Sh::kTile, r, j * kBN + r, it.len, bk, it.number, t);
                     fence_proxy_async_smem();
                 }
-                // p of 32 keys at a time into the first 64 columns of S; the products of the first 64 keys may
-                // start while the others are on their way
-                const float2 sl2 = make_float2(sl, sl), nm2 = make_float2(-m_run, -m_run);
-                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t pk[16];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float2 y = __ffma2_rn(make_float2(__uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1])), sl2, nm2);
-                        const float2 p = (e & 3) < kFmaPairs ? exp2_fma(y) : make_float2(fast_exp2(y.x), fast_exp2(y.y));
-                        sum[e & 1] = __fadd2_rn(sum[e & 1], p);
-                        pk[e] = pack_16x2<F16>(p.x, p.y);
-                    }
-                    if (c == 2) {
-                        tmem_wait_st();
-                        tc_fence_before();
-                        mbar_arrive(&bk->p_full[t][0]);
-                    }
-                    tmem_st16(tS + c * 16, pk);
-                }
-                l_run += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-                tmem_wait_st();
-                tc_fence_before();
-                mbar_arrive(&bk->p_full[t][1]);
+                any_tile<D, F16>(tS, tO, sl, j == n - 1 ? pos - j * kBN : kBN, j > 0, m_run, l_run, bk->p_full[t]);
             }
             slot0 += 2 * nj;
             if (!ok || n == 0) continue;
