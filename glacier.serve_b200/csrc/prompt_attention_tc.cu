@@ -13,14 +13,14 @@
 //  * warps 0-3 and 4-7, one warpgroup per query tile, one thread per query row: scores from tensor
 //    memory, causal mask on the last key tile, online softmax with lazy rescaling (O is rescaled
 //    only where the running maximum grows by more than 2^8, so p stays below 2^8), P back into tensor
-//    memory; at the end O / l through shared memory to whole rows of the output.
+//    memory; at the end O / l to the output.
 //  * warps 8 and 9, one per query tile: one thread of each issues the tile's products (one thread for
 //    both spent a third of its time on waits and commits with the tensor pipe idle), in turns, so that
 //    the two tiles' softmaxes do not fall together.  S of key tile
 //    j + 1 overwrites P of tile j, so it is issued behind P V of tile j (products of one thread execute
 //    in issue order), and a warpgroup that sees S of tile j + 1 knows that O holds P V of tile j:
 //    rescaling needs no further barrier.
-//  * warp 10: one thread loads Q, and K and V tiles in turn through a ring of 4 slots (TMA, 128-byte
+//  * warp 10: loads Q, and K and V tiles in turn through a ring of 4 slots (TMA, 128-byte
 //    swizzle, no multicast).
 //  * warp 11: finds the next item while the block works on this one.  The grid holds every item, the
 //    longest of a prompt first; a running block takes over blocks that have not started
@@ -49,21 +49,22 @@ constexpr int kEarly = 64;                        // keys whose P V starts befor
 constexpr int kMmaWarp = 8, kLoadWarp = 10, kPlanWarp = 11;  // kMmaWarp + t issues query tile t's products
 constexpr int kThreads = 384;
 constexpr int kRing = 4;
+constexpr int kItems = 1;                         // item slots: the next item, while the block works on one
+constexpr int kPrefix = 1024;                     // prompts whose tile counts fit a block's shared memory
 constexpr uint32_t kTmemCols = 512;               // S0 S1 O0 O1, 128 columns each
 constexpr uint32_t kColS = 0, kColO = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleLog2 = 8.f;
 constexpr uint32_t kPolls = 1u << 24;
-constexpr uint32_t kPlanNs = 1000, kLoadNs = 200, kMmaNs = 0, kSoftNs = 0;
+constexpr uint32_t kPlanNs = 100, kLoadNs = 40, kMmaNs = 0, kSoftNs = 0;
 
 template <int D>
 struct Shape {
     static constexpr uint32_t kHalf = kBN * 128;            // 128 rows x 64 dims
     static constexpr int kHalves = D / 64;
     static constexpr uint32_t kTile = kHalves * kHalf;      // a Q, K or V tile
-    static constexpr uint32_t kStage = kBM * 64;            // output staging of a warpgroup: 128 rows x 32 dims
-    static constexpr uint32_t kData = 2 * kTile + kRing * kTile + 2 * kStage;
-    static constexpr uint32_t kBytes = kData + 13312 + 1024;  // + bookkeeping + alignment
+    static constexpr uint32_t kData = 2 * kTile + kRing * kTile;
+    static constexpr uint32_t kBytes = kData + 17664 + 1024;  // + bookkeeping + alignment
 };
 
 struct Item {
@@ -75,13 +76,13 @@ struct Item {
 };
 
 struct Book {
-    uint64_t q_full, q_empty;
+    uint64_t q_full[2], q_empty[2];
     uint64_t ring_full[kRing], ring_empty[kRing];
     uint64_t s_full[2], p_full[2][2], o_full[2];  // p_full: of the first kEarly keys, and of the others
-    uint64_t item_full, item_empty;
+    uint64_t item_full[kItems], item_empty[kItems];
     uint64_t steal, drained[2], turn[2];
     alignas(16) uint32_t response[4];
-    Item item;
+    Item item[kItems];
     uint32_t tmem;
     int abort;
     // Not-finite values taken out of a query tile's last key tile: for each dim the first position with
@@ -90,8 +91,9 @@ struct Book {
     // one item ahead of the second, which reads both tiles' entries, and not more.
     int poisoned[2][2];  // one more than the number of the item that the entries are of
     unsigned long long poison[2][2][3][128];
+    int tiles_before[kPrefix + 1];  // of each prompt (batch <= kPrefix)
 };
-static_assert(sizeof(Book) <= 13312, "bookkeeping");
+static_assert(sizeof(Book) <= 17664, "bookkeeping");
 
 constexpr uint32_t idesc_16(int m, int n, bool b_mn_major, bool f16) {
     const uint32_t fmt = f16 ? 0u : 1u;
@@ -146,6 +148,12 @@ __device__ __forceinline__ int stolen_block(const uint32_t* response) {
         : "r"(smem_u32(response))
         : "memory");
     return ok ? static_cast<int>(x) : -1;
+}
+
+__device__ __forceinline__ void store_sector(void* p, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
 }
 
 template <bool F16>
@@ -204,6 +212,30 @@ __device__ __forceinline__ float exp2_in_order(float x) {
     asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Not-finite values that were taken out of the last key tiles (of the own one and, for the second query
+// tile, of the first's), back into the row at position `pos`, whose thread has just stored it.
+template <int D, bool F16>
+__device__ __noinline__ void put_back(const Book* bk, int number, int t, int pos, uint8_t* out) {
+    for (int e = 0; e < D; ++e) {
+        bool sees[3];
+        for (int k = 0; k < 3; ++k) {
+            sees[k] = false;
+            for (int u = 0; u <= t; ++u) {
+                const unsigned long long w = *reinterpret_cast<const volatile unsigned long long*>(&bk->poison[number & 1][u][k][e]);
+                sees[k] |= static_cast<uint32_t>(w >> 32) == ~static_cast<uint32_t>(number) && static_cast<uint32_t>(pos) >= static_cast<uint32_t>(w);
+            }
+        }
+        if (!sees[0] && !sees[1] && !sees[2]) continue;
+        uint16_t* p = reinterpret_cast<uint16_t*>(out) + e;
+        const uint32_t was = *p;
+        float x = F16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(was))) : __uint_as_float(was << 16);
+        if (sees[0]) x = __uint_as_float(0x7fffffffu);
+        if (sees[1]) x += INFINITY;
+        if (sees[2]) x += -INFINITY;
+        *p = static_cast<uint16_t>(pack_16x2<F16>(x, 0.f));
+    }
+}
+
 // Weights of 32 keys: p = 2^(sl s - m) of s[0 .. 31], in pairs of the inputs' type; `sum` grows by them.
 // In groups of 8 pairs, the exponentials of a group one after the other and their sums behind them: left
 // to itself the compiler put each sum next to its exponential, and a warp has only one other on its
@@ -323,18 +355,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t{1023});
     uint8_t* sQ = smem;
     uint8_t* sRing = sQ + 2 * Sh::kTile;
-    uint8_t* sStage = sRing + kRing * Sh::kTile;
     Book* bk = reinterpret_cast<Book*>(smem + Sh::kData);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
-        mbar_init(&bk->q_full, 1);
-        mbar_init(&bk->q_empty, 2);
         for (int i = 0; i < kRing; ++i) {
             mbar_init(&bk->ring_full[i], 1);
             mbar_init(&bk->ring_empty[i], 2);
         }
         for (int t = 0; t < 2; ++t) {
+            mbar_init(&bk->q_full[t], 1);
+            mbar_init(&bk->q_empty[t], 1);
             mbar_init(&bk->s_full[t], 1);
             mbar_init(&bk->p_full[t][0], 128);
             mbar_init(&bk->p_full[t][1], 128);
@@ -343,8 +374,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&bk->o_full[t], 1);
             bk->poisoned[t][0] = bk->poisoned[t][1] = 0;
         }
-        mbar_init(&bk->item_full, 1);
-        mbar_init(&bk->item_empty, 11);  // both warpgroups' warps, the issuers, the loader
+        for (int i = 0; i < kItems; ++i) {
+            mbar_init(&bk->item_full[i], 1);
+            mbar_init(&bk->item_empty[i], 11);  // both warpgroups' warps, the issuers, the loader
+        }
         mbar_init(&bk->steal, 1);
         bk->abort = 0;
         fence_mbar_init();
@@ -362,15 +395,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     fewer_registers<56>();
     if (warp == kPlanWarp) {
         // ---------------- items ----------------
+        // The blocks of the grid stand for the tiles in descending order, all heads of a tile in a row;
+        // behind the last tile some stand for none (the host knows only total and batch).
         if (blockIdx.x == 0) check_prompts(a, lane, 32);
+        if (lane == 0) steal_block(bk->response, &bk->steal);  // the first answer is on its way meanwhile
+        const int numbers = static_cast<int>(gridDim.x / a.n_heads);
+        const bool listed = a.batch <= kPrefix;
+        const int tiles = listed ? list_prompt_tiles<kRows>(a, bk->tiles_before) : 0;
         int block = blockIdx.x, published = 0;
-        uint32_t asked = 0;
-        const int last = static_cast<int>(gridDim.x / a.n_heads) - 1;
+        uint32_t answers = 0;
+        bool asking = true;
         while (true) {
             PromptTile pt;
             const int x = block / a.n_heads;
-            const bool found = block >= 0 && find_prompt_tile<kRows>(a, last - x, pt);
+            bool found = false;
+            if (block >= 0) found = listed ? x < tiles && listed_prompt_tile<kRows>(a, bk->tiles_before, tiles - 1 - x, pt)
+                                           : find_prompt_tile<kRows>(a, numbers - 1 - x, pt);
             if (found || block < 0) {
+                const int is = published % kItems;
+                if (published >= kItems && !(ok = __all_sync(~0u, wait(&bk->item_empty[is], (published / kItems - 1) & 1, bk, kPlanNs)))) break;
                 if (lane == 0) {
                     Item it{};
                     if (found) {
@@ -382,65 +425,76 @@ __global__ void __launch_bounds__(kThreads, 1)
                         it.n[1] = it.len - it.q0 > kBM ? it.n[0] + 1 : 0;
                         it.number = published;
                     }
-                    bk->item = it;
-                    mbar_arrive(&bk->item_full);
+                    bk->item[is] = it;
+                    mbar_arrive(&bk->item_full[is]);
                 }
                 __syncwarp();
                 if (block < 0) break;
-                // the next item is fetched once every warp has begun this one
-                if (!(ok = __all_sync(~0u, wait(&bk->item_empty, published & 1, bk, kPlanNs)))) break;
                 ++published;
             }
-            if (lane == 0) steal_block(bk->response, &bk->steal);
-            __syncwarp();
-            if (!(ok = __all_sync(~0u, mbar_wait(&bk->steal, asked & 1)))) break;  // the answer must land, come what may
-            ++asked;
+            if (!(ok = __all_sync(~0u, mbar_wait(&bk->steal, answers & 1)))) break;
+            ++answers;
             block = stolen_block(bk->response);
+            asking = block >= 0;
             __syncwarp();
-            fence_proxy_async_smem();  // the answer has been read before the next one is written
+            if (asking) {
+                fence_proxy_async_smem();  // the answer has been read before the next one is written
+                if (lane == 0) steal_block(bk->response, &bk->steal);
+            }
+            __syncwarp();
         }
+        // an answer still on its way must land before the block's shared memory goes away
+        if (!ok && asking && lane == 0) mbar_wait(&bk->steal, answers & 1);
         if (!ok && lane == 0) {
             bk->abort = 1;
             atomicOr(a.err, kErrWaitTimeout);
         }
     } else if (warp == kLoadWarp) {
         // ---------------- TMA ----------------
-        if (lane == 0) {
-            uint32_t slot = 0, q_loads = 0;
-            for (uint32_t i = 0;; ++i) {
-                if (!(ok = wait(&bk->item_full, i & 1, bk, kLoadNs))) break;
-                const Item it = bk->item;
-                mbar_arrive(&bk->item_empty);
-                if (it.n[0] == 0) break;
-                if (i > 0 && !(ok = wait(&bk->q_empty, (i - 1) & 1, bk, kLoadNs))) break;
-                const int kv = it.head / (a.n_heads / a.heads_kv);
-                const int row = static_cast<int>(it.row0) + it.q0;
-                mbar_arrive_expect_tx(&bk->q_full, it.n[1] ? 2 * Sh::kTile : Sh::kTile);
-                ++q_loads;
-                const int nj = it.n[1] ? it.n[1] : it.n[0];
-                auto load = [&](uint8_t* dst, const CUtensorMap* tm, int head, int r, uint64_t* bar) {
-#pragma unroll
-                    for (int h = 0; h < Sh::kHalves; ++h) tma_load_3d(dst + h * Sh::kHalf, tm, h * 64, head, r, bar);
-                };
-                load(sQ, &tmq, it.head, row, &bk->q_full);
-                for (int j = 0; j < 2 * nj; ++j) {  // K of tile j / 2, then V
-                    const int s = slot % kRing;
-                    if (slot >= kRing && !(ok = wait(&bk->ring_empty[s], (slot / kRing - 1) & 1, bk, kLoadNs))) break;
-                    mbar_arrive_expect_tx(&bk->ring_full[s], Sh::kTile);
-                    load(sRing + s * Sh::kTile, (j & 1) ? &tmv : &tmk, kv, static_cast<int>(it.row0) + (j >> 1) * kBN, &bk->ring_full[s]);
-                    ++slot;
-                    if (j == 0 && it.n[1]) load(sQ + Sh::kTile, &tmq, it.head, row + kBM, &bk->q_full);
-                }
-                if (!ok) break;
+        // Each copy by lanes of its own, one per box of 128 rows x 64 dims: a copy holds its thread for some
+        // hundred cycles.
+        uint32_t slot = 0, q_loads[2] = {0, 0};
+        auto empty = [&](uint64_t* bar, uint32_t parity) { return __all_sync(~0u, wait(bar, parity, bk, kLoadNs)) != 0; };
+        auto load = [&](uint8_t* dst, const CUtensorMap* tm, int head, int row, uint64_t* bar) {
+            if (lane == 0) mbar_arrive_expect_tx(bar, Sh::kTile);
+            __syncwarp();  // the expected bytes before the first of them
+            if (lane < Sh::kHalves) tma_load_3d(dst + lane * Sh::kHalf, tm, lane * 64, head, row, bar);
+        };
+        for (uint32_t i = 0;; ++i) {
+            const int is = i % kItems;
+            if (!(ok = empty(&bk->item_full[is], (i / kItems) & 1))) break;
+            const Item it = bk->item[is];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bk->item_empty[is]);
+            if (it.n[0] == 0) break;
+            const int kv = it.head / (a.n_heads / a.heads_kv), row = static_cast<int>(it.row0);
+            const int nj = it.n[1] ? it.n[1] : it.n[0];
+            auto load_q = [&](int t) {
+                if (it.n[t] == 0) return true;
+                if (q_loads[t] > 0 && !empty(&bk->q_empty[t], (q_loads[t] - 1) & 1)) return false;
+                load(sQ + t * Sh::kTile, &tmq, it.head, row + it.q0 + t * kBM, &bk->q_full[t]);
+                ++q_loads[t];
+                return true;
+            };
+            if (!(ok = load_q(0))) break;
+            for (int j = 0; j < 2 * nj; ++j) {  // K of tile j / 2, then V
+                const int s = slot % kRing;
+                if (slot >= kRing && !(ok = empty(&bk->ring_empty[s], (slot / kRing - 1) & 1))) break;
+                load(sRing + s * Sh::kTile, (j & 1) ? &tmv : &tmk, kv, row + (j >> 1) * kBN, &bk->ring_full[s]);
+                ++slot;
+                if (j == 0 && !(ok = load_q(1))) break;
             }
-            if (!ok) {
-                bk->abort = 1;
-                atomicOr(a.err, kErrWaitTimeout);
-                // every copy must land before the block's shared memory goes away
-                if (q_loads) mbar_wait(&bk->q_full, (q_loads - 1) & 1);
-                for (uint32_t s = slot > kRing ? slot - kRing : 0; s < slot; ++s) mbar_wait(&bk->ring_full[s % kRing], (s / kRing) & 1);
-            }
+            if (!ok) break;
         }
+        if (!ok && lane == 0) {
+            bk->abort = 1;
+            atomicOr(a.err, kErrWaitTimeout);
+            // every copy must land before the block's shared memory goes away
+            for (int t = 0; t < 2; ++t)
+                if (q_loads[t]) mbar_wait(&bk->q_full[t], (q_loads[t] - 1) & 1);
+            for (uint32_t s = slot > kRing ? slot - kRing : 0; s < slot; ++s) mbar_wait(&bk->ring_full[s % kRing], (s / kRing) & 1);
+        }
+        __syncwarp();
     } else {
         // ---------------- products of query tile t ----------------
         // The whole warp keeps the loop, so that ring positions and descriptors are the same for all its
@@ -456,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t k_desc = umma_desc_sw128(smem_u32(sRing), 16, 1024);
         const uint64_t v_desc = umma_desc_sw128(smem_u32(sRing), Sh::kHalf, 1024);
         uint32_t slot = 0;          // ring position of the next tile
-        uint32_t p_count = 0, turns = 0;
+        uint32_t p_count = 0, q_count = 0, turns = 0;
         auto ready = [&](uint64_t* bar, uint32_t parity) { return __all_sync(~0u, wait(bar, parity, bk, kMmaNs)) != 0; };
         auto full = [&](uint32_t at) { return ready(&bk->ring_full[at % kRing], (at / kRing) & 1); };
         auto scores = [&](uint32_t at) {  // S = Q K^T
@@ -469,24 +523,25 @@ __global__ void __launch_bounds__(kThreads, 1)
             umma_commit(&bk->s_full[t]);
         };
         for (uint32_t i = 0;; ++i) {
-            if (!(ok = ready(&bk->item_full, i & 1))) break;
-            const int n0 = __shfl_sync(~0u, bk->item.n[0], 0), n1 = __shfl_sync(~0u, bk->item.n[1], 0);
+            const int is = i % kItems;
+            if (!(ok = ready(&bk->item_full[is], (i / kItems) & 1))) break;
+            const int n0 = __shfl_sync(~0u, bk->item[is].n[0], 0), n1 = __shfl_sync(~0u, bk->item[is].n[1], 0);
             __syncwarp();
-            if (issuer) mbar_arrive(&bk->item_empty);
+            if (issuer) mbar_arrive(&bk->item_empty[is]);
             if (n0 == 0) break;
             const int n = t ? n1 : n0, nj = n1 ? n1 : n0;
             // a slot is free when both tiles are done with it: behind this tile's products so far, or,
             // where it has none, as soon as the slot is filled
-            if (!(ok = ready(&bk->q_full, i & 1) && full(slot))) break;
+            if (!(ok = (n == 0 || ready(&bk->q_full[t], q_count & 1)) && full(slot))) break;
+            if (n > 0) ++q_count;
             tc_fence_after();
             if (issuer) {
                 if (n > 0) {
                     scores(slot);
                     umma_commit(&bk->ring_empty[slot % kRing]);
-                    if (n == 1) umma_commit(&bk->q_empty);
+                    if (n == 1) umma_commit(&bk->q_empty[t]);
                 } else {
                     mbar_arrive(&bk->ring_empty[slot % kRing]);
-                    mbar_arrive(&bk->q_empty);
                 }
             }
             __syncwarp();
@@ -528,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mbar_arrive(&bk->turn[t ^ 1]);
                     umma_commit(&bk->ring_empty[vs % kRing]);
                     if (more) umma_commit(&bk->ring_empty[ks % kRing]);
-                    if (j + 2 == n) umma_commit(&bk->q_empty);
+                    if (j + 2 == n) umma_commit(&bk->q_empty[t]);
                 }
                 __syncwarp();
             }
@@ -554,26 +609,27 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t s_count = 0, o_count = 0;
         uint32_t slot0 = 0;  // ring position of the item's first tile
         for (uint32_t i = 0; ok; ++i) {
-            if (!(ok = __all_sync(~0u, wait(&bk->item_full, i & 1, bk, kSoftNs)))) break;
-            const Item it = bk->item;
+            const int is = i % kItems;
+            if (!(ok = __all_sync(~0u, wait(&bk->item_full[is], (i / kItems) & 1, bk, kSoftNs)))) break;
+            const Item it = bk->item[is];
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bk->item_empty);
+            if (lane == 0) mbar_arrive(&bk->item_empty[is]);
             if (it.n[0] == 0) break;
             const int n = t ? it.n[1] : it.n[0];
             const int nj = it.n[1] ? it.n[1] : it.n[0];
             const int pos = it.q0 + t * kBM + r;
             float m_run = -INFINITY, l_run = 0.f;
             for (int j = 0; j < n; ++j) {
-                if (!(ok = __all_sync(~0u, wait(&bk->s_full[t], s_count & 1, bk, kSoftNs)))) break;
-                ++s_count;
-                tc_fence_after();
-                if (j > 0 && j < n - 1 && middle_tile<F16>(tS, sl, m_run, l_run, bk->p_full[t])) continue;
-                if (j == n - 1) {
+                if (j == n - 1) {  // while the scores are on their way
                     const uint32_t vs = slot0 + 2 * j + 1;
                     if (!(ok = __all_sync(~0u, wait(&bk->ring_full[vs % kRing], (vs / kRing) & 1, bk, kSoftNs)))) break;
                     clean_values<D, F16>(sRing + (vs % kRing) * Sh::kTile, r, j * kBN + r, it.len, bk, it.number, t);
                     fence_proxy_async_smem();
                 }
+                if (!(ok = __all_sync(~0u, wait(&bk->s_full[t], s_count & 1, bk, kSoftNs)))) break;
+                ++s_count;
+                tc_fence_after();
+                if (j > 0 && j < n - 1 && middle_tile<F16>(tS, sl, m_run, l_run, bk->p_full[t])) continue;
                 any_tile<D, F16>(tS, tO, sl, j == n - 1 ? pos - j * kBN : kBN, j > 0, m_run, l_run, bk->p_full[t]);
             }
             slot0 += 2 * nj;
@@ -596,57 +652,25 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int rows = min(kBM, it.len - it.q0 - t * kBM);
             const int64_t row = it.row0 + it.q0 + t * kBM;
             if (a.lse && r < rows) a.lse[(row + r) * a.n_heads + it.head] = (top + log2f(total)) * 0.6931471805599453f;
-            uint8_t* stage = sStage + t * Sh::kStage + (warp & 3) * (32 * 64);
-            uint8_t* out = static_cast<uint8_t*>(a.out) + (row * a.n_heads + it.head) * (D * 2);
-            const int64_t out_row = static_cast<int64_t>(a.n_heads) * (D * 2);
-            const volatile int* tags = bk->poisoned[it.number & 1];
-            const bool bad = tags[0] == it.number + 1 || (t && tags[1] == it.number + 1);
+            // each row from its thread, in whole 32-byte sectors
+            uint8_t* out = static_cast<uint8_t*>(a.out) + ((row + r) * a.n_heads + it.head) * (D * 2);
 #pragma unroll 1
-            for (int h = 0; h < D / 32; ++h) {
-                uint32_t o[32];
-                tmem_ld32(tO + h * 32, o);
+            for (int h = 0; h < D / 64; ++h) {
+                uint32_t o[2][32];
+                tmem_ld32(tO + h * 64, o[0]);
+                tmem_ld32(tO + h * 64 + 32, o[1]);
                 tmem_wait_ld();
-                if (bad) {
-                    // rows that see a not-finite value taken out of the last key tiles: of the own one
-                    // and, for the second query tile, of the first's
-#pragma unroll 1
-                    for (int e = 0; e < 32; ++e) {
-                        bool sees[3];
-                        for (int k = 0; k < 3; ++k) {
-                            sees[k] = false;
-                            for (int u = 0; u <= t; ++u) {
-                                const unsigned long long w = bk->poison[it.number & 1][u][k][h * 32 + e];
-                                sees[k] |= static_cast<uint32_t>(w >> 32) == ~static_cast<uint32_t>(it.number) &&
-                                           static_cast<uint32_t>(pos) >= static_cast<uint32_t>(w);
-                            }
-                        }
-                        float add = 0.f;
-                        if (sees[0] || (sees[1] && sees[2])) add = __uint_as_float(0x7fffffffu);
-                        else if (sees[1]) add = INFINITY;
-                        else if (sees[2]) add = -INFINITY;
 #pragma unroll
-                        for (int q = 0; q < 32; ++q)
-                            if (q == e) o[q] = __float_as_uint(__uint_as_float(o[q]) + add);
-                    }
-                }
-                __syncwarp();  // the last piece's rows have been read from the stage
+                for (int c = 0; c < 64; c += 16) {
+                    uint32_t w[8];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        w[e] = pack_16x2<F16>(__uint_as_float(o[c * 8 + e * 2]) * inv, __uint_as_float(o[c * 8 + e * 2 + 1]) * inv);
-                    *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-                __syncwarp();
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int rr = k * 8 + (lane >> 2), c = lane & 3;
-                    const uint4 w = *reinterpret_cast<const uint4*>(stage + rr * 64 + ((c ^ ((rr >> 1) & 3)) << 4));
-                    const int tr = (warp & 3) * 32 + rr;
-                    if (tr < rows) *reinterpret_cast<uint4*>(out + tr * out_row + h * 64 + c * 16) = w;
+                    for (int e = 0; e < 8; ++e)
+                        w[e] = pack_16x2<F16>(__uint_as_float(o[c >> 5][(c & 31) + 2 * e]) * inv, __uint_as_float(o[c >> 5][(c & 31) + 2 * e + 1]) * inv);
+                    if (r < rows) store_sector(out + h * 128 + c * 2, w);
                 }
             }
+            const volatile int* tags = bk->poisoned[it.number & 1];
+            if ((tags[0] == it.number + 1 || (t && tags[1] == it.number + 1)) && r < rows) put_back<D, F16>(bk, it.number, t, pos, out);
             tc_fence_before();
         }
         if (!ok) {

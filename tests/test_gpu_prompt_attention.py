@@ -224,3 +224,13 @@ def test_refusals(cuda):
     assert pool.last_launch_count == 0
     pool.close()
     other.close()
+
+
+@pytest.mark.parametrize("batch", [33, 1024, 1025, 3000])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_many_prompts(cuda, dtype, batch):
+    """Batches on both sides of what a block lists, empty prompts and one-token ones among them."""
+    rng = np.random.default_rng(batch)
+    lens = rng.choice([0, 0, 1, 2, 7, 130, 257], batch).tolist()
+    q, k, v, cu = _inputs(lens, 2, 1, 64, 64, dtype, seed=batch)
+    _check(q, k, v, cu, 0.125)
