@@ -22,8 +22,8 @@
 //    rescaling needs no further barrier.
 //  * warp 10: loads Q, and K and V tiles in turn through a ring of 4 slots (TMA, 128-byte
 //    swizzle, no multicast).
-//  * warp 11: finds the next item while the block works on this one.  The grid holds every item, the
-//    longest of a prompt first; a running block takes over blocks that have not started
+//  * warp 11: finds the next item while the block works on this one.  The grid holds every item, those
+//    with the most keys first; a running block takes over blocks that have not started
 //    (clusterlaunchcontrol), so the next item's loads and first scores overlap this one's end.
 // Values that no row may see (keys behind a prompt's end, and not-finite values of keys that some rows
 // of the last key tile do not see) are taken out of the V tile before its product; the rows that do see
@@ -50,7 +50,6 @@ constexpr int kMmaWarp = 8, kLoadWarp = 10, kPlanWarp = 11;  // kMmaWarp + t iss
 constexpr int kThreads = 384;
 constexpr int kRing = 4;
 constexpr int kItems = 1;                         // item slots: the next item, while the block works on one
-constexpr int kPrefix = 1024;                     // prompts whose tile counts fit a block's shared memory
 constexpr uint32_t kTmemCols = 512;               // S0 S1 O0 O1, 128 columns each
 constexpr uint32_t kColS = 0, kColO = 256;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -64,7 +63,7 @@ struct Shape {
     static constexpr int kHalves = D / 64;
     static constexpr uint32_t kTile = kHalves * kHalf;      // a Q, K or V tile
     static constexpr uint32_t kData = 2 * kTile + kRing * kTile;
-    static constexpr uint32_t kBytes = kData + 17664 + 1024;  // + bookkeeping + alignment
+    static constexpr uint32_t kBytes = kData + 27648 + 1024;  // + bookkeeping + alignment
 };
 
 struct Item {
@@ -91,9 +90,9 @@ struct Book {
     // one item ahead of the second, which reads both tiles' entries, and not more.
     int poisoned[2][2];  // one more than the number of the item that the entries are of
     unsigned long long poison[2][2][3][128];
-    int tiles_before[kPrefix + 1];  // of each prompt (batch <= kPrefix)
+    PromptList list;  // where batch <= kListed
 };
-static_assert(sizeof(Book) <= 17664, "bookkeeping");
+static_assert(sizeof(Book) <= 27648, "bookkeeping");
 
 constexpr uint32_t idesc_16(int m, int n, bool b_mn_major, bool f16) {
     const uint32_t fmt = f16 ? 0u : 1u;
@@ -384,9 +383,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = threadIdx.x; i < 2 * 2 * 3 * 128; i += kThreads) (&bk->poison[0][0][0][0])[i] = ~0ull;
     if (warp == kMmaWarp) tmem_alloc(&bk->tmem, kTmemCols);
+    const bool listed = a.batch <= kListed;
+    if (listed) count_prompt_tiles<kRows>(a, bk->list, threadIdx.x, kThreads);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (listed) {
+        sort_prompts(a, bk->list, threadIdx.x, kThreads);
+        __syncthreads();
+    }
     const uint32_t tmem = bk->tmem;
     bool ok = true;
 
@@ -395,13 +400,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     fewer_registers<56>();
     if (warp == kPlanWarp) {
         // ---------------- items ----------------
-        // The blocks of the grid stand for the tiles in descending order, all heads of a tile in a row;
-        // behind the last tile some stand for none (the host knows only total and batch).
+        // The blocks of the grid stand for the tiles, those with the most keys first (with a batch too large
+        // to be listed, for each prompt), all heads of a tile in a row; some stand for none: the host knows
+        // only total and batch.
         if (blockIdx.x == 0) check_prompts(a, lane, 32);
         if (lane == 0) steal_block(bk->response, &bk->steal);  // the first answer is on its way meanwhile
         const int numbers = static_cast<int>(gridDim.x / a.n_heads);
-        const bool listed = a.batch <= kPrefix;
-        const int tiles = listed ? list_prompt_tiles<kRows>(a, bk->tiles_before) : 0;
+        const int tiles = listed ? sum_prompt_levels(a, bk->list) : 0;
         int block = blockIdx.x, published = 0;
         uint32_t answers = 0;
         bool asking = true;
@@ -409,8 +414,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             PromptTile pt;
             const int x = block / a.n_heads;
             bool found = false;
-            if (block >= 0) found = listed ? x < tiles && listed_prompt_tile<kRows>(a, bk->tiles_before, tiles - 1 - x, pt)
-                                           : find_prompt_tile<kRows>(a, numbers - 1 - x, pt);
+            if (block >= 0 && listed) {
+                found = x < tiles;
+                if (found) listed_prompt_tile(a, bk->list, x, pt);
+            } else if (block >= 0) {
+                found = find_prompt_tile<kRows>(a, numbers - 1 - x, pt);
+            }
             if (found || block < 0) {
                 const int is = published % kItems;
                 if (published >= kItems && !(ok = __all_sync(~0u, wait(&bk->item_empty[is], (published / kItems - 1) & 1, bk, kPlanNs)))) break;

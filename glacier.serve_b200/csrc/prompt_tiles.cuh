@@ -39,45 +39,70 @@ __device__ __forceinline__ bool find_prompt_tile(const PromptArgs& a, int x, Pro
     return out.tile >= 0 && static_cast<int64_t>(out.tile) * T < out.len;
 }
 
-// The same with the tile counts of all prompts listed first, by one warp: before[b] = tiles of the
-// prompts before b (before[batch] = all of them, returned).  A prompt whose range is bad has none.
+// The tiles of up to kListed prompts in descending order of their keys: first every prompt's last tile
+// that is as far from its start as any, then the next nearer ones.  With the prompts sorted by tile count,
+// c_0 >= c_1 >= ..., c_k tiles deep the first k + 1 of them still have one: levels c_{k+1} .. c_k - 1 hold
+// (k + 1) (c_k - c_{k+1}) tiles, so a tile number finds its k by a search over their sums.
+constexpr int kListed = 1024;
+struct PromptList {
+    int count[kListed];        // tiles of each prompt (none where its range is bad)
+    int sorted[kListed + 1];   // in descending order, then 0
+    int before[kListed + 1];   // tiles of the levels above c_k
+    unsigned short order[kListed];
+};
+// Three steps, a block barrier behind each of the first two.
 template <int T>
-__device__ __forceinline__ int list_prompt_tiles(const PromptArgs& a, int* before) {
+__device__ __forceinline__ void count_prompt_tiles(const PromptArgs& a, PromptList& l, int thread, int threads) {
+    for (int b = thread; b < a.batch; b += threads) {
+        const int begin = __ldg(a.cu + b), end = __ldg(a.cu + b + 1);
+        l.count[b] = begin >= 0 && end >= begin && end <= a.total ? (end - begin) / T + ((end - begin) % T != 0) : 0;
+    }
+}
+__device__ __forceinline__ void sort_prompts(const PromptArgs& a, PromptList& l, int thread, int threads) {
+    for (int b = thread; b < a.batch; b += threads) {
+        const int c = l.count[b];
+        int rank = 0;
+        for (int o = 0; o < a.batch; ++o) {
+            const int x = l.count[o];
+            rank += x > c || (x == c && o < b);
+        }
+        l.sorted[rank] = c;
+        l.order[rank] = static_cast<unsigned short>(b);
+    }
+    if (thread == 0) l.sorted[a.batch] = 0;
+}
+// By one warp; returns the number of tiles.
+__device__ __forceinline__ int sum_prompt_levels(const PromptArgs& a, PromptList& l) {
     const int lane = threadIdx.x & 31;
     int sum = 0;
     for (int base = 0; base < a.batch; base += 32) {
-        const int b = base + lane;
-        int n = 0;
-        if (b < a.batch) {
-            const int begin = __ldg(a.cu + b), end = __ldg(a.cu + b + 1);
-            if (begin >= 0 && end >= begin && end <= a.total) n = (end - begin + T - 1) / T;
-        }
+        const int k = base + lane;
+        const int n = k < a.batch ? (k + 1) * (l.sorted[k] - l.sorted[k + 1]) : 0;
         int inc = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int y = __shfl_up_sync(~0u, inc, o);
             if (lane >= o) inc += y;
         }
-        if (b < a.batch) before[b] = sum + inc - n;
+        if (k < a.batch) l.before[k] = sum + inc - n;
         sum += __shfl_sync(~0u, inc, 31);
     }
-    if (lane == 0) before[a.batch] = sum;
     __syncwarp();
     return sum;
 }
-template <int T>
-__device__ __forceinline__ bool listed_prompt_tile(const PromptArgs& a, const int* before, int tile, PromptTile& out) {
-    int lo = 0, hi = a.batch;  // the last prompt with before[b] <= tile: those behind it without tiles share its end
+__device__ __forceinline__ void listed_prompt_tile(const PromptArgs& a, const PromptList& l, int tile, PromptTile& out) {
+    int lo = 0, hi = a.batch;  // the last k with before[k] <= tile: those with as many tiles as the next hold none
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (before[mid] <= tile) lo = mid;
+        if (l.before[mid] <= tile) lo = mid;
         else hi = mid;
     }
-    const int begin = __ldg(a.cu + lo), end = __ldg(a.cu + lo + 1);
+    const int in = tile - l.before[lo], level = in / (lo + 1);
+    const int b = l.order[in - level * (lo + 1)];
+    const int begin = __ldg(a.cu + b), end = __ldg(a.cu + b + 1);
     out.row0 = begin;
     out.len = end - begin;
-    out.tile = tile - before[lo];
-    return true;
+    out.tile = l.sorted[lo] - 1 - level;
 }
 
 // Looks every prompt's range over, whether or not a tile of it is ever searched for.
