@@ -74,37 +74,50 @@ __device__ __forceinline__ void store8_as(void* base, int dtype, int64_t at, con
     else store8(static_cast<__half*>(base) + at, x, 1.f);
 }
 
-// x += bias, element by element (biases need no alignment).
-__device__ __forceinline__ void add8(const float* bias, float (&x)[8]) {
+// 8 floats of a bias or norm weight (whose address need not be a multiple of 16 bytes).
+__device__ __forceinline__ void weights8(const float* w, float (&x)[8]) {
+    if ((reinterpret_cast<uintptr_t>(w) & 15) == 0) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(w)), b = __ldg(reinterpret_cast<const float4*>(w) + 1);
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] += __ldg(bias + e);
+        for (int e = 0; e < 8; ++e) x[e] = __ldg(w + e);
+    }
 }
 
 // T: the type of q, k and v; KV: the arena's.
 template <typename T, typename KV>
 __global__ void __launch_bounds__(kThreads) mrope_append_kernel(const ArenaGeom g, const __grid_constant__ MropeParams a, const int tokens) {
     pdl_launch_dependents();  // the decode that follows waits for this grid before reading q or the arena
-    __shared__ float2 turn[kMaxTokens * kMropeMaxPairs];  // (cos, sin) * mscale of each token's pairs
-    __shared__ int64_t slot_of[kMaxTokens];
+    __shared__ __align__(16) float2 turn[kMaxTokens * kMropeMaxPairs];  // (cos, sin) * mscale of each token's pairs
+    __shared__ int64_t k_row[kMaxTokens], v_row[kMaxTokens];            // each token's row of head 0 in the arenas, -1: not stored
     const int n_tok = a.dyn_tok ? min(__ldg(a.dyn_tok), a.n_tok) : a.n_tok;
     const int t0 = blockIdx.x * tokens;
     const int nt = min(tokens, n_tok - t0);
     if (nt <= 0) return;
     const int half = a.rope_dim / 2;
+    // The tables are in the parameters, but are read as memory: 32 different addresses of the constant
+    // bank are 32 reads one after the other.
+    const float* inv_freq = a.inv_freq;
+    const uint8_t* axis = a.axis;
+    asm volatile("" : "+l"(inv_freq), "+l"(axis));
     for (int i = threadIdx.x; i < nt * half; i += kThreads) {
         const int t = i / half, j = i - t * half;
-        const int pos = __ldg(a.positions + a.axis[j] * a.pos_stride + t0 + t);
+        const int pos = __ldg(a.positions + axis[j] * a.pos_stride + t0 + t);
         float s, c;
-        rope_sincos_f64(static_cast<double>(pos) * static_cast<double>(a.inv_freq[j]), s, c);
+        rope_sincos_f64(static_cast<double>(pos) * static_cast<double>(inv_freq[j]), s, c);
         turn[i] = make_float2(c * a.mscale, s * a.mscale);
     }
     if (threadIdx.x < nt) {
-        int64_t s = __ldg(a.slots + t0 + threadIdx.x);
+        const int64_t s = __ldg(a.slots + t0 + threadIdx.x);
+        k_row[threadIdx.x] = v_row[threadIdx.x] = -1;
         if (s >= static_cast<int64_t>(g.total_blocks) * g.block_size) {
             atomicOr(a.err, kErrBadSlot);
-            s = -1;
+        } else if (s >= 0) {
+            const int64_t blk = s / g.block_size, off = s - blk * g.block_size;
+            k_row[threadIdx.x] = blk * g.k_block_stride + a.layer * g.k_layer_stride + off * g.head_dim;
+            v_row[threadIdx.x] = blk * g.v_block_stride + a.layer * g.v_layer_stride + off * g.v_head_dim;
         }
-        slot_of[threadIdx.x] = s;
     }
     __syncthreads();
 
@@ -132,8 +145,13 @@ __global__ void __launch_bounds__(kThreads) mrope_append_kernel(const ArenaGeom 
         load8(src + ib, y);
         const float* bias = is_q ? a.q_bias : a.k_bias;
         if (bias) {
-            add8(bias + h * d + ia, x);
-            add8(bias + h * d + ib, y);
+            float w[8];
+            weights8(bias + h * d + ia, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] += w[e];
+            weights8(bias + h * d + ib, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] += w[e];
         }
         if (a.q_norm || a.k_norm) {  // the same for the whole grid; a row without a weight ignores the sum
             float p = 0.f;
@@ -142,32 +160,40 @@ __global__ void __launch_bounds__(kThreads) mrope_append_kernel(const ArenaGeom 
             for (int o = tpr >> 1; o >= 1; o >>= 1) p += __shfl_xor_sync(~0u, p, o);
             if (const float* w = is_q ? a.q_norm : a.k_norm) {
                 const float inv = 1.f / sqrtf(p / static_cast<float>(d) + a.eps);
+                float v[8];
+                weights8(w + ia, v);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    x[e] *= inv * __ldg(w + ia + e);
-                    y[e] *= inv * __ldg(w + ib + e);
-                }
+                for (int e = 0; e < 8; ++e) x[e] *= inv * v[e];
+                weights8(w + ib, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] *= inv * v[e];
             }
         }
         if (!live) continue;
         if (u < half) {  // all 8 pairs, or none
-            const float2* w = turn + t * half + u;
+            const float4* w4 = reinterpret_cast<const float4*>(turn + t * half + u);
+            float c[8], s[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float4 w = w4[e];
+                c[2 * e] = w.x, s[2 * e] = w.y, c[2 * e + 1] = w.z, s[2 * e + 1] = w.w;
+            }
             if (neox) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float p = x[e];
-                    x[e] = p * w[e].x - y[e] * w[e].y;
-                    y[e] = y[e] * w[e].x + p * w[e].y;
+                    x[e] = p * c[e] - y[e] * s[e];
+                    y[e] = y[e] * c[e] + p * s[e];
                 }
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) {
-                    const float2 w0 = w[e / 2], w1 = w[4 + e / 2];
+                    const int e0 = e / 2, e1 = 4 + e / 2;
                     const float p = x[e], q = y[e];
-                    x[e] = p * w0.x - x[e + 1] * w0.y;
-                    x[e + 1] = x[e + 1] * w0.x + p * w0.y;
-                    y[e] = q * w1.x - y[e + 1] * w1.y;
-                    y[e + 1] = y[e + 1] * w1.x + q * w1.y;
+                    x[e] = p * c[e0] - x[e + 1] * s[e0];
+                    x[e + 1] = x[e + 1] * c[e0] + p * s[e0];
+                    y[e] = q * c[e1] - y[e + 1] * s[e1];
+                    y[e + 1] = y[e + 1] * c[e1] + q * s[e1];
                 }
             }
         }
@@ -176,11 +202,8 @@ __global__ void __launch_bounds__(kThreads) mrope_append_kernel(const ArenaGeom 
             store8_as(out, a.out_dtype, at + ia, x);
             store8_as(out, a.out_dtype, at + ib, y);
         }
-        const int64_t slot = slot_of[t];
-        if (!is_q && slot >= 0) {
-            const int64_t blk = slot / g.block_size;
-            KV* dst = static_cast<KV*>(g.k) + blk * g.k_block_stride + a.layer * g.k_layer_stride + h * g.k_head_stride +
-                      (slot - blk * g.block_size) * d;
+        if (!is_q && k_row[t] >= 0) {
+            KV* dst = static_cast<KV*>(g.k) + k_row[t] + h * g.k_head_stride;
             const float inv = g.k_inv ? __ldg(g.k_inv + a.layer * hk + h) : 1.f;
             store8(dst + ia, x, inv);
             store8(dst + ib, y, inv);
@@ -194,14 +217,15 @@ __global__ void __launch_bounds__(kThreads) mrope_append_kernel(const ArenaGeom 
         const int64_t tok = t0 + t;
         float x[8];
         load8(static_cast<const T*>(a.v) + tok * a.v_ts + h * a.v_hs + e, x);
-        if (a.v_bias) add8(a.v_bias + h * dv + e, x);
+        if (a.v_bias) {
+            float w[8];
+            weights8(a.v_bias + h * dv + e, w);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] += w[k];
+        }
         if (a.v_out) store8_as(a.v_out, a.out_dtype, (tok * hk + h) * dv + e, x);
-        const int64_t slot = slot_of[t];
-        if (slot < 0) continue;
-        const int64_t blk = slot / g.block_size;
-        KV* dst = static_cast<KV*>(g.v) + blk * g.v_block_stride + a.layer * g.v_layer_stride + h * g.v_head_stride +
-                  (slot - blk * g.block_size) * dv + e;
-        store8(dst, x, g.v_inv ? __ldg(g.v_inv + a.layer * hk + h) : 1.f);
+        if (v_row[t] >= 0)
+            store8(static_cast<KV*>(g.v) + v_row[t] + h * g.v_head_stride + e, x, g.v_inv ? __ldg(g.v_inv + a.layer * hk + h) : 1.f);
     }
 }
 
