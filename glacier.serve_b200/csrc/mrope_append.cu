@@ -74,20 +74,16 @@ __device__ __forceinline__ void store8_as(void* base, int dtype, int64_t at, con
     else store8(static_cast<__half*>(base) + at, x, 1.f);
 }
 
-// 8 floats of a bias or norm weight (whose address need not be a multiple of 16 bytes).
+// 8 floats of a bias or norm weight, from a 16-byte boundary.
 __device__ __forceinline__ void weights8(const float* w, float (&x)[8]) {
-    if ((reinterpret_cast<uintptr_t>(w) & 15) == 0) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(w)), b = __ldg(reinterpret_cast<const float4*>(w) + 1);
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = __ldg(w + e);
-    }
+    const float4 a = __ldg(reinterpret_cast<const float4*>(w)), b = __ldg(reinterpret_cast<const float4*>(w) + 1);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
 }
 
-// T: the type of q, k and v; KV: the arena's.
-template <typename T, typename KV>
-__global__ void __launch_bounds__(kThreads) mrope_append_kernel(const ArenaGeom g, const __grid_constant__ MropeParams a, const int tokens) {
+// T: the type of q, k and v; KV: the arena's; NORM: q or k has a norm weight.  Bound by issued
+// instructions as much as by memory: what does not depend on the token is computed once per head row.
+template <typename T, typename KV, bool NORM>
+__global__ void __launch_bounds__(kThreads, 4) mrope_append_kernel(const ArenaGeom g, const __grid_constant__ MropeParams a, const int tokens) {
     pdl_launch_dependents();  // the decode that follows waits for this grid before reading q or the arena
     __shared__ __align__(16) float2 turn[kMaxTokens * kMropeMaxPairs];  // (cos, sin) * mscale of each token's pairs
     __shared__ int64_t k_row[kMaxTokens], v_row[kMaxTokens];            // each token's row of head 0 in the arenas, -1: not stored
@@ -123,97 +119,104 @@ __global__ void __launch_bounds__(kThreads) mrope_append_kernel(const ArenaGeom 
 
     const int d = g.head_dim, hk = g.heads_kv, lane = threadIdx.x & 31;
     const int tpr = d / 16;  // lanes of a head row: 2, 4, 8 or 16
-    const int rows = a.n_heads + hk;
-    const int units = nt * rows * tpr;
+    const int tpr_log2 = 31 - __clz(tpr);
+    const int units = (a.n_heads + hk) * tpr;
     const bool neox = a.style == GKV_ROPE_NEOX;
-    // whole warps run every pass: the norm's sums cross lanes
+    // A lane takes one place of one head, of one token after the other.  Whole warps run every pass: the
+    // norm's sums cross lanes.
     for (int i = threadIdx.x; i - lane < units; i += kThreads) {
         const bool live = i < units;
-        const int row = live ? i / tpr : 0, u = live ? (i - row * tpr) * 8 : 0;  // pairs u .. u + 7 of d / 2
-        const int t = row / rows, r = row - t * rows;
+        const int r = live ? i >> tpr_log2 : 0, u = live ? (i - (r << tpr_log2)) * 8 : 0;  // pairs u .. u + 7 of d / 2
         const bool is_q = r < a.n_heads;
         const int h = is_q ? r : r - a.n_heads;
-        const int64_t tok = t0 + t;
         // NEOX: 8 first elements of pairs, then their 8 partners; the unrotated elements [R, d) pair
         // up as halves too.  Interleaved: 16 adjacent elements.  R is a multiple of 16, so a vector
         // lies on one side of it.
         const int ia = neox ? (u < half ? u : u + half) : 2 * u;
         const int ib = neox ? (u < half ? u + half : u + d / 2) : 2 * u + 8;
-        const T* src = is_q ? static_cast<const T*>(a.q) + tok * a.q_ts + h * a.q_hs : static_cast<const T*>(a.k) + tok * a.k_ts + h * a.k_hs;
-        float x[8], y[8];
-        load8(src + ia, x);
-        load8(src + ib, y);
+        const int64_t ts = is_q ? a.q_ts : a.k_ts;
+        const T* src = (is_q ? static_cast<const T*>(a.q) + h * a.q_hs : static_cast<const T*>(a.k) + h * a.k_hs) + t0 * ts;
         const float* bias = is_q ? a.q_bias : a.k_bias;
-        if (bias) {
-            float w[8];
-            weights8(bias + h * d + ia, w);
+        if (bias) bias += h * d;
+        const float* norm = NORM ? (is_q ? a.q_norm : a.k_norm) : nullptr;
+        void* out = is_q ? a.q_out : a.k_out;
+        const int out_stride = (is_q ? a.n_heads : hk) * d;
+        int64_t at = static_cast<int64_t>(t0) * out_stride + h * d;
+        KV* k_dst = static_cast<KV*>(g.k) + h * g.k_head_stride;
+        const float k_inv = !is_q && g.k_inv ? __ldg(g.k_inv + a.layer * hk + h) : 1.f;
+        const float4* w4 = reinterpret_cast<const float4*>(turn + u);
+#pragma unroll 1
+        for (int t = 0; t < nt; ++t, src += ts, at += out_stride, w4 += half / 2) {
+            float x[8], y[8];
+            load8(src + ia, x);
+            load8(src + ib, y);
+            if (bias) {
+                float w[8];
+                weights8(bias + ia, w);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] += w[e];
-            weights8(bias + h * d + ib, w);
+                for (int e = 0; e < 8; ++e) x[e] += w[e];
+                weights8(bias + ib, w);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] += w[e];
-        }
-        if (a.q_norm || a.k_norm) {  // the same for the whole grid; a row without a weight ignores the sum
-            float p = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) p = fmaf(x[e], x[e], fmaf(y[e], y[e], p));
-            for (int o = tpr >> 1; o >= 1; o >>= 1) p += __shfl_xor_sync(~0u, p, o);
-            if (const float* w = is_q ? a.q_norm : a.k_norm) {
-                const float inv = 1.f / sqrtf(p / static_cast<float>(d) + a.eps);
-                float v[8];
-                weights8(w + ia, v);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] *= inv * v[e];
-                weights8(w + ib, v);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] *= inv * v[e];
+                for (int e = 0; e < 8; ++e) y[e] += w[e];
             }
-        }
-        if (!live) continue;
-        if (u < half) {  // all 8 pairs, or none
-            const float4* w4 = reinterpret_cast<const float4*>(turn + t * half + u);
-            float c[8], s[8];
+            if constexpr (NORM) {
+                float p = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float4 w = w4[e];
-                c[2 * e] = w.x, s[2 * e] = w.y, c[2 * e + 1] = w.z, s[2 * e + 1] = w.w;
-            }
-            if (neox) {
+                for (int e = 0; e < 8; ++e) p = fmaf(x[e], x[e], fmaf(y[e], y[e], p));
+                for (int o = tpr >> 1; o >= 1; o >>= 1) p += __shfl_xor_sync(~0u, p, o);
+                if (norm) {
+                    const float inv = 1.f / sqrtf(p / static_cast<float>(d) + a.eps);
+                    float w[8];
+                    weights8(norm + ia, w);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float p = x[e];
-                    x[e] = p * c[e] - y[e] * s[e];
-                    y[e] = y[e] * c[e] + p * s[e];
-                }
-            } else {
+                    for (int e = 0; e < 8; ++e) x[e] *= inv * w[e];
+                    weights8(norm + ib, w);
 #pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    const int e0 = e / 2, e1 = 4 + e / 2;
-                    const float p = x[e], q = y[e];
-                    x[e] = p * c[e0] - x[e + 1] * s[e0];
-                    x[e + 1] = x[e + 1] * c[e0] + p * s[e0];
-                    y[e] = q * c[e1] - y[e + 1] * s[e1];
-                    y[e + 1] = y[e + 1] * c[e1] + q * s[e1];
+                    for (int e = 0; e < 8; ++e) y[e] *= inv * w[e];
                 }
             }
-        }
-        if (void* out = is_q ? a.q_out : a.k_out) {
-            const int64_t at = (tok * (is_q ? a.n_heads : hk) + h) * d;
-            store8_as(out, a.out_dtype, at + ia, x);
-            store8_as(out, a.out_dtype, at + ib, y);
-        }
-        if (!is_q && k_row[t] >= 0) {
-            KV* dst = static_cast<KV*>(g.k) + k_row[t] + h * g.k_head_stride;
-            const float inv = g.k_inv ? __ldg(g.k_inv + a.layer * hk + h) : 1.f;
-            store8(dst + ia, x, inv);
-            store8(dst + ib, y, inv);
+            if (!live) continue;
+            if (u < half) {  // all 8 pairs, or none
+                float c[8], s[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float4 w = w4[e];
+                    c[2 * e] = w.x, s[2 * e] = w.y, c[2 * e + 1] = w.z, s[2 * e + 1] = w.w;
+                }
+                if (neox) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float p = x[e];
+                        x[e] = p * c[e] - y[e] * s[e];
+                        y[e] = y[e] * c[e] + p * s[e];
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        const int e0 = e / 2, e1 = 4 + e / 2;
+                        const float p = x[e], q = y[e];
+                        x[e] = p * c[e0] - x[e + 1] * s[e0];
+                        x[e + 1] = x[e + 1] * c[e0] + p * s[e0];
+                        y[e] = q * c[e1] - y[e + 1] * s[e1];
+                        y[e + 1] = y[e + 1] * c[e1] + q * s[e1];
+                    }
+                }
+            }
+            if (out) {
+                store8_as(out, a.out_dtype, at + ia, x);
+                store8_as(out, a.out_dtype, at + ib, y);
+            }
+            if (!is_q && k_row[t] >= 0) {
+                store8(k_dst + k_row[t] + ia, x, k_inv);
+                store8(k_dst + k_row[t] + ib, y, k_inv);
+            }
         }
     }
     // v: 8 elements per lane
-    const int dv = g.v_head_dim, vpr = dv / 8;
-    for (int i = threadIdx.x; i < nt * hk * vpr; i += kThreads) {
-        const int row = i / vpr, e = (i - row * vpr) * 8;
-        const int t = row / hk, h = row - t * hk;
+    const int dv = g.v_head_dim, vpr = dv / 8, v_units = hk * vpr;
+    for (int i = threadIdx.x; i < nt * v_units; i += kThreads) {
+        const int t = i / v_units, r = i - t * v_units;
+        const int h = r / vpr, e = (r - h * vpr) * 8;
         const int64_t tok = t0 + t;
         float x[8];
         load8(static_cast<const T*>(a.v) + tok * a.v_ts + h * a.v_hs + e, x);
@@ -233,8 +236,9 @@ template <typename T, typename KV>
 cudaError_t launch_typed(const ArenaGeom& g, const MropeParams& p, cudaStream_t st) {
     // one token per block until the card is full
     const int tokens = p.n_tok <= 148 * 8 ? 1 : kMaxTokens;
-    const int64_t blocks = (static_cast<int64_t>(p.n_tok) + tokens - 1) / tokens;
-    mrope_append_kernel<T, KV><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(g, p, tokens);
+    const unsigned blocks = static_cast<unsigned>((static_cast<int64_t>(p.n_tok) + tokens - 1) / tokens);
+    if (p.q_norm || p.k_norm) mrope_append_kernel<T, KV, true><<<blocks, kThreads, 0, st>>>(g, p, tokens);
+    else mrope_append_kernel<T, KV, false><<<blocks, kThreads, 0, st>>>(g, p, tokens);
     return cudaGetLastError();
 }
 

@@ -1146,6 +1146,10 @@ int step_mrope_append(Pool* p, int32_t layer, const gkv_qkv_io* io, int32_t n_to
             ((reinterpret_cast<uintptr_t>(io->d_q_out) | reinterpret_cast<uintptr_t>(io->d_k_out) |
               reinterpret_cast<uintptr_t>(io->d_v_out)) & 15))
             return set_error(GKV_EINVAL, "q/k/v and the outputs need head rows on 16-byte boundaries");
+        if (pro && ((reinterpret_cast<uintptr_t>(pro->d_q_bias) | reinterpret_cast<uintptr_t>(pro->d_k_bias) |
+                     reinterpret_cast<uintptr_t>(pro->d_v_bias) | reinterpret_cast<uintptr_t>(pro->d_q_norm) |
+                     reinterpret_cast<uintptr_t>(pro->d_k_norm)) & 15))
+            return set_error(GKV_EINVAL, "biases and norm weights need 16-byte boundaries");
         const bool in_place = io->d_q_out == io->d_q && io->out_dtype == io->dtype && (n_heads == 1 || io->q_head_stride == d) &&
                               (n_tok == 1 || io->q_tok_stride == static_cast<int64_t>(n_heads) * d);
         const void* in[] = {io->d_q, io->d_k, io->d_v};

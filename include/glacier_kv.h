@@ -364,7 +364,8 @@ typedef struct gkv_qkv_io {
  * count, read on the device, and the launch can be captured: n_tok is then the arrays' capacity (at
  * least the step's max_tokens; rows past it in a later replayed step are left out).  Rows behind the
  * step's last are left alone.  head_dim must be 32, 64, 128 or 256
- * (GKV_EUNSUPPORTED).  Element strides and pointers must keep every head row 16-byte aligned, and
+ * (GKV_EUNSUPPORTED).  Element strides and pointers must keep every head row 16-byte aligned,
+ * the prologue's pointers too, and
  * d_q_out may only overlap d_q as said above, the other outputs no input (GKV_EINVAL for the
  * alignment, and for an output at the address of another tensor). */
 GKV_API int gkv_mrope_append(gkv_pool* pool, int32_t layer, const gkv_qkv_io* io, int32_t n_tok,

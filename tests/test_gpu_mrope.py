@@ -203,6 +203,11 @@ def test_refusals(cuda):
         pool.mrope_append(0, wide[:, 1:257].view(4, 4, 64), k, v, pos, rope, out)  # off the 16-byte boundary
     with pytest.raises(bad):
         pool.mrope_append(0, wide[:, :256].view(4, 4, 64), k, v, pos, rope, out)   # rows off it
+    odd = torch.zeros(4 * 64 + 1, device="cuda")[1:]
+    with pytest.raises(bad):
+        pool.mrope_append(0, q, k, v, pos, rope, out, q_bias=odd)
+    with pytest.raises(bad):
+        pool.mrope_append(0, q, k, v, pos, rope, out, k_norm=odd[:64])
     with pytest.raises(ValueError):
         pool.mrope_append(0, q, k.half(), v, pos, rope, out)
     with pytest.raises(ValueError):
