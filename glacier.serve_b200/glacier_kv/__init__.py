@@ -103,31 +103,49 @@ def _stream(stream, device: int) -> Optional[int]:
     return stream.cuda_stream
 
 
+# The checks below stand on the path of single tokens, where a call's own time counts: one look at each
+# property of a tensor, and the explanation only once something is wrong.
+
 def _dev(t, name: str, dtypes, device: int, shape=None):
-    """Data pointer of a dense CUDA tensor on `device` of one of `dtypes` (and of `shape`, None = any size)."""
-    if not (t.is_cuda and t.dtype in dtypes and t.is_contiguous() and t.device.index == device):
+    """Data pointer of a dense CUDA tensor on `device` of one of `dtypes` (and of `shape`, None = any)."""
+    if t.get_device() != device or t.dtype not in dtypes or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {' / '.join(str(x) for x in dtypes)} tensor on cuda:{device}")
-    if shape is not None and (t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape))):
-        raise ValueError(f"{name} must have shape {tuple('*' if n is None else n for n in shape)}, not {tuple(t.shape)}")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
     return t.data_ptr()
 
 
 def _rows(t, name: str, dtype, device: int, shape):
     """(pointer, token stride, head stride) of a [tokens, heads, dim] CUDA tensor with dense head rows."""
-    if not (t.is_cuda and t.dtype == dtype and t.device.index == device):
+    if t.get_device() != device or t.dtype != dtype:
         raise ValueError(f"{name} must be a {dtype} tensor on cuda:{device}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} must have shape {shape}, not {tuple(t.shape)}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
     s = t.stride()
     if s[2] != 1 and shape[2] > 1:
         raise ValueError(f"the head rows of {name} must be dense")
     return t.data_ptr(), s[0], s[1]
 
 
-def _q_dtypes():
-    import torch
+class _Torch:
+    """torch's types, looked up once (the package does not need torch for its host side)."""
 
-    return {torch.float32: GKV_DTYPE_F32, torch.bfloat16: GKV_DTYPE_BF16, torch.float16: GKV_DTYPE_F16}
+    kinds = None
+
+    @classmethod
+    def load(cls):
+        import torch
+
+        cls.f32, cls.i32, cls.current_stream = (torch.float32,), (torch.int32,), torch.cuda.current_stream
+        cls.kinds = {torch.float32: GKV_DTYPE_F32, torch.bfloat16: GKV_DTYPE_BF16, torch.float16: GKV_DTYPE_F16}
+        return cls.kinds
+
+
+def _queue(stream, device: int) -> int:
+    """The stream of a call on a pool with a device arena."""
+    if stream is None:
+        return _Torch.current_stream(device).cuda_stream
+    return stream if isinstance(stream, int) else stream.cuda_stream
 
 
 def _f32_dev(t, name: str):
@@ -389,15 +407,14 @@ class PagedBlockPool:
         """gkv_step_build: block tables, slot mapping, positions and work list of a step from the
         request lengths in `io`, on the GPU (static step layout).  `batch` and `n_new_blocks`
         default to the sizes of io's tensors."""
-        d = io._desc
         if io.device != self.device:
             raise ValueError(f"the step's arrays are on cuda:{io.device}, the pool on cuda:{self.device}")
         b = io.max_batch if batch is None else batch
         n = io.max_new_blocks if n_new_blocks is None else n_new_blocks
         if not 0 <= b <= io.max_batch or not 0 <= n <= io.max_new_blocks:
             raise ArgumentOutOfRangeError(GKV_EINVAL, f"batch {b} / n_new_blocks {n} exceed the arrays ({io.max_batch} / {io.max_new_blocks})")
-        d.n_new_blocks = n
-        _check(lib.gkv_step_build(self._h, io._ref, b, _stream(stream, self.device)))
+        io._desc.n_new_blocks = n
+        _check(lib.gkv_step_build(self._h, io._ref, b, _queue(stream, self.device)))
 
     def mrope_append(self, layer: int, q, k, v, positions, rope: "MultiAxisRope", q_out, k_out=None, v_out=None, q_bias=None,
                      k_bias=None, v_bias=None, q_norm=None, k_norm=None, eps: float = 1e-6, stream=None) -> None:
@@ -406,52 +423,56 @@ class PagedBlockPool:
         type (float32, bfloat16, float16), strided as the parts of a fused projection are; positions
         [n_axes, n_tok] int32 CUDA; q_out dense (q itself for in place), k_out / v_out dense or None,
         all of one type; biases and norm weights float32 CUDA or None."""
-        kinds, dev = _q_dtypes(), self.device
-        if q.dtype not in kinds or q_out.dtype not in kinds or q.dim() != 3:
+        kinds, dev = _Torch.kinds or _Torch.load(), self.device
+        kind, out = q.dtype, q_out.dtype
+        if kind not in kinds or out not in kinds or q.dim() != 3:
             raise ValueError("q and q_out must be [n_tok, n_heads, head_dim] float32, bfloat16 or float16 CUDA tensors")
-        n, nh = q.shape[0], q.shape[1]
+        n, nh, _ = q.shape
         hk, d, dv = self._heads_kv, self._head_dim, self._v_head_dim
-        o = (q_out.dtype,)
-        qp, qt, qh = _rows(q, "q", q.dtype, dev, (n, nh, d))
-        kp, kt, kh = _rows(k, "k", q.dtype, dev, (n, hk, d))
-        vp, vt, vh = _rows(v, "v", q.dtype, dev, (n, hk, dv))
+        o, f, keys = (out,), _Torch.f32, (n, hk, d)
+        qp, qt, qh = _rows(q, "q", kind, dev, (n, nh, d))
+        kp, kt, kh = _rows(k, "k", kind, dev, keys)
+        vp, vt, vh = _rows(v, "v", kind, dev, (n, hk, dv))
         io = _lib.gkv_qkv_io(qp, kp, vp, _dev(q_out, "q_out", o, dev, (n, nh, d)),
-                             None if k_out is None else _dev(k_out, "k_out", o, dev, (n, hk, d)),
+                             None if k_out is None else _dev(k_out, "k_out", o, dev, keys),
                              None if v_out is None else _dev(v_out, "v_out", o, dev, (n, hk, dv)),
-                             qt, qh, kt, kh, vt, vh, kinds[q.dtype], kinds[q_out.dtype])
-        import torch
+                             qt, qh, kt, kh, vt, vh, kinds[kind], kinds[out])
 
-        pp = _dev(positions, "positions", (torch.int32,), dev, (rope.n_axes, n))
-        f = (torch.float32,)
-        opt = lambda t, name, m: None if t is None else _dev(t.view(-1), name, f, dev, (m,))  # noqa: E731
-        pro = _lib.gkv_qkv_prologue(opt(q_bias, "q_bias", nh * d), opt(k_bias, "k_bias", hk * d), opt(v_bias, "v_bias", hk * dv),
-                                    opt(q_norm, "q_norm", d), opt(k_norm, "k_norm", d), eps)
-        _check(lib.gkv_mrope_append(self._h, layer, io, n, nh, pp, n, rope._desc, pro, _stream(stream, dev)))
+        def weights(t, name, m):
+            if t.numel() != m:
+                raise ValueError(f"{name} must have {m} values, not {t.numel()}")
+            return _dev(t, name, f, dev)
+
+        pro = _lib.gkv_qkv_prologue(None if q_bias is None else weights(q_bias, "q_bias", nh * d),
+                                    None if k_bias is None else weights(k_bias, "k_bias", hk * d),
+                                    None if v_bias is None else weights(v_bias, "v_bias", hk * dv),
+                                    None if q_norm is None else weights(q_norm, "q_norm", d),
+                                    None if k_norm is None else weights(k_norm, "k_norm", d), eps)
+        _check(lib.gkv_mrope_append(self._h, layer, io, n, nh, _dev(positions, "positions", _Torch.i32, dev, (rope.n_axes, n)), n,
+                                    rope._desc, pro, _queue(stream, dev)))
 
     def prompt_attention(self, q, k, v, cu_seqlens, out, scale: float, sinks=None, lse=None, stream=None) -> None:
         """Causal attention of packed whole prompts over their own k and v (gkv_prompt_attention):
         q [total, n_heads, head_dim], k, v [total, heads_kv, ...] CUDA tensors of one type (float32,
         bfloat16, float16) with strides; cu_seqlens [batch + 1] int32 CUDA; out dense [total, n_heads,
         v_head_dim] of the same type; sinks [n_heads] and lse [total, n_heads] float32 CUDA or None."""
-        kinds, dev = _q_dtypes(), self.device
-        if q.dtype not in kinds or q.dim() != 3:
+        kinds, dev = _Torch.kinds or _Torch.load(), self.device
+        kind = q.dtype
+        if kind not in kinds or q.dim() != 3:
             raise ValueError("q must be a [total, n_heads, head_dim] float32, bfloat16 or float16 CUDA tensor")
-        import torch
-
-        n, nh = q.shape[0], q.shape[1]
+        n, nh, _ = q.shape
         hk, d, dv = self._heads_kv, self._head_dim, self._v_head_dim
-        f = (torch.float32,)
-        qp, qt, qh = _rows(q, "q", q.dtype, dev, (n, nh, d))
-        kp, kt, kh = _rows(k, "k", q.dtype, dev, (n, hk, d))
-        vp, vt, vh = _rows(v, "v", q.dtype, dev, (n, hk, dv))
-        cp = _dev(cu_seqlens, "cu_seqlens", (torch.int32,), dev, (None,))
-        if cu_seqlens.shape[0] < 1:
+        qp, qt, qh = _rows(q, "q", kind, dev, (n, nh, d))
+        kp, kt, kh = _rows(k, "k", kind, dev, (n, hk, d))
+        vp, vt, vh = _rows(v, "v", kind, dev, (n, hk, dv))
+        cp = _dev(cu_seqlens, "cu_seqlens", _Torch.i32, dev)
+        if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
             raise ValueError("cu_seqlens must hold batch + 1 entries")
-        desc = _lib.gkv_prompt_desc(qp, kp, vp, _dev(out, "out", (q.dtype,), dev, (n, nh, dv)),
-                                    None if lse is None else _dev(lse, "lse", f, dev, (n, nh)),
-                                    None if sinks is None else _dev(sinks, "sinks", f, dev, (nh,)), cp,
-                                    qt, qh, kt, kh, vt, vh, cu_seqlens.shape[0] - 1, n, nh, kinds[q.dtype], scale)
-        _check(lib.gkv_prompt_attention(self._h, desc, _stream(stream, dev)))
+        desc = _lib.gkv_prompt_desc(qp, kp, vp, _dev(out, "out", (kind,), dev, (n, nh, dv)),
+                                    None if lse is None else _dev(lse, "lse", _Torch.f32, dev, (n, nh)),
+                                    None if sinks is None else _dev(sinks, "sinks", _Torch.f32, dev, (nh,)), cp,
+                                    qt, qh, kt, kh, vt, vh, cu_seqlens.shape[0] - 1, n, nh, kinds[kind], scale)
+        _check(lib.gkv_prompt_attention(self._h, desc, _queue(stream, dev)))
 
     def kv_append(self, layer: int, k, v, stream=None) -> None:
         """k [n_tok, heads_kv, head_dim], v [n_tok, heads_kv, v_head_dim] float32 CUDA."""
@@ -549,12 +570,15 @@ class StepBuffers:
     def __init__(self, block_tables, ctx_lens, new_lens, new_blocks, max_tokens: int):
         import torch
 
-        i32, dev = (torch.int32,), block_tables.device.index
-        b = ctx_lens.shape[0]
+        _Torch.load()
+        i32, dev = _Torch.i32, block_tables.get_device()
+        if dev < 0 or block_tables.dim() != 2 or ctx_lens.dim() != 1 or new_blocks.dim() != 1:
+            raise ValueError("block_tables must be [max_batch, max_blocks], the lengths [max_batch] and new_blocks [n], all int32 CUDA")
+        b, width = block_tables.shape
         if max_tokens < 0:
             raise ArgumentOutOfRangeError(GKV_EINVAL, f"negative max_tokens {max_tokens}")
         ptrs = [_dev(ctx_lens, "ctx_lens", i32, dev, (b,)), _dev(new_lens, "new_lens", i32, dev, (b,)),
-                _dev(new_blocks, "new_blocks", i32, dev, (None,)), _dev(block_tables, "block_tables", i32, dev, (b, None))]
+                _dev(new_blocks, "new_blocks", i32, dev), _dev(block_tables, "block_tables", i32, dev)]
         self.block_tables, self.ctx_lens, self.new_lens, self.new_blocks = block_tables, ctx_lens, new_lens, new_blocks
         make = lambda n, t=torch.int32: torch.zeros(n, dtype=t, device=block_tables.device)  # noqa: E731
         self.ctx_out, self.cu_new, self.counts = make(b), make(b + 1), make(2)
@@ -562,7 +586,7 @@ class StepBuffers:
         self.device, self.max_batch, self.max_new_blocks, self.max_tokens = dev, b, new_blocks.shape[0], max_tokens
         self._desc = _lib.gkv_step_io(*ptrs, self.ctx_out.data_ptr(), self.cu_new.data_ptr(), self.slots.data_ptr(),
                                       self.positions.data_ptr(), self.counts.data_ptr(), self.max_new_blocks,
-                                      block_tables.shape[1], max_tokens)
+                                      width, max_tokens)
         self._ref = C.byref(self._desc)
 
 
