@@ -164,7 +164,8 @@ struct StepWorkspace {
     DecodeWork work{};
     const int64_t* d_slots = nullptr;
     bool uploaded = false;
-    bool built = false;          // the step came from gkv_step_build and no launch has followed it
+    bool device_step = false;    // the step came from gkv_step_build
+    bool built = false;          // and no launch has followed it
     std::vector<int32_t> h_ctx;  // ctx_lens of the uploaded step
     WorkList wl;                 // the uploaded step's work list (kept for its capacity)
     // chunked prefill: pinned + device buffer of its work items / work list, and q in the

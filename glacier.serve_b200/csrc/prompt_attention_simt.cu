@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(kThreads) prompt_simt_kernel(const PromptArgs 
         const float top = fmaxf(m[r], sink);
         const float base = top == -INFINITY ? 0.f : top;
         const float alpha = fast_exp2(m[r] - base);
-        const float total = sum * alpha + fast_exp2(sink - base);
+        const float total = sum * alpha + (sink == base ? 1.f : fast_exp2(sink - base));  // also where both are infinite
         const float inv = alpha / total;
         const int row = ti * R + r;
         if (row >= nq) continue;

@@ -653,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 top = fmaxf(m_run, sink);
                 const float base = top == -INFINITY ? 0.f : top;
                 const float alpha = fast_exp2(m_run - base);
-                total = l_run * alpha + fast_exp2(sink - base);
+                total = l_run * alpha + (sink == base ? 1.f : fast_exp2(sink - base));  // also where both are infinite
                 inv = alpha / total;
             } else {
                 inv = 1.f / l_run;

@@ -552,7 +552,7 @@ int step_upload(Pool* p, const int32_t* tables, int32_t batch, int32_t max_block
     ws.n_tok = n_tok;
     ws.up_max_blocks = max_blocks;
     ws.uploaded = true;
-    ws.built = false;
+    ws.built = ws.device_step = false;
     return GKV_OK;
 }
 
@@ -574,6 +574,9 @@ int step_build(Pool* p, const gkv_step_io* io, int32_t batch, cudaStream_t st) {
         return set_error(GKV_EINVAL, "ctx_out must not be ctx_lens or new_lens (every block of the kernel reads those)");
     const int64_t workers = static_cast<int64_t>(ws.n_ctas_max) * ws.cfg.warps;
     const int64_t n_seg = static_cast<int64_t>(ws.max_batch) * p->desc.heads_kv;
+    if (p->desc.heads_kv >= 1 << 10 || n_seg >= 1 << 20 || workers >= 1 << 14)
+        return set_error(GKV_EUNSUPPORTED, "step building is not built for %d requests of %d kv heads and %lld workers", ws.max_batch,
+                         p->desc.heads_kv, static_cast<long long>(workers));
     const MetaLayout L = meta_layout(ws.max_tokens, ws.max_batch, 0, workers + n_seg, workers, n_seg);
     if (L.total > ws.meta_cap || static_cast<size_t>(n_seg) * 12 > ws.meta_cap || L.total > 0x7fffffff)
         return set_error(GKV_ESTATE, "static step buffer too small");
@@ -630,7 +633,7 @@ int step_build(Pool* p, const gkv_step_io* io, int32_t batch, cudaStream_t st) {
     ws.n_tok = io->max_tokens;
     ws.up_max_blocks = io->table_stride;
     ws.uploaded = true;
-    ws.built = true;
+    ws.built = ws.device_step = true;
     return GKV_OK;
 }
 
@@ -1026,6 +1029,8 @@ int step_rope_append(Pool* p, int32_t layer, float* d_q, const float* d_k, const
                      const gkv_qkv_prologue* pro, cudaStream_t st) {
     StepWorkspace& ws = p->ws;
     if (!ws.uploaded) return set_error(GKV_ESTATE, "no step uploaded (call gkv_upload_step first)");
+    if (ws.device_step)
+        return set_error(GKV_ESTATE, "the rows of a step built on the device are known there alone (use gkv_mrope_append)");
     if (!rope) return set_error(GKV_EINVAL, "rope description is NULL");
     if (layer < 0 || layer >= p->desc.layers)
         return set_error(GKV_EINVAL, "layer %d outside [0, %d)", layer, p->desc.layers);

@@ -155,7 +155,7 @@ __device__ __forceinline__ bool served(const StepBuildArgs& a, const Request& r,
 // The stream of units over the live requests (those with a context): request k's head h spans units
 // [pre[k] + h * span, ... + span), span = kSegmentCost + its chunks, pre[k + 1] = pre[k] + H span.
 // Quotients come from estimates in 32-bit floating point, put right by one exact product to each
-// side: they are below 2^13 (workers) and 2^10 (heads), so an estimate is off by less than one.
+// side: they are below 2^14 (workers) and 2^10 (heads), so an estimate is off by less than one.
 struct Units {
     const uint32_t* pre;  // [live + 1]
     int live, H, n;       // n: workers
@@ -164,7 +164,7 @@ struct Units {
 
     // first unit of worker w: floor(w * total / n)
     __device__ __forceinline__ uint32_t begin(int w) const {
-        const uint32_t x = r * static_cast<uint32_t>(w);  // below 2^26
+        const uint32_t x = r * static_cast<uint32_t>(w);  // below 2^28
         uint32_t e = static_cast<uint32_t>(static_cast<float>(x) * inv_n);
         e -= e * n > x;
         e += (e + 1) * n <= x;
@@ -458,7 +458,7 @@ __global__ void order_kernel() {}
 cudaError_t launch_step_build(const StepBuildArgs& a, cudaStream_t st) {
     if (a.batch < 0 || a.batch > kMaxBuildBatch) return cudaErrorInvalidValue;
     const int64_t n_seg = static_cast<int64_t>(a.batch) * a.heads_kv;
-    if (a.n_workers < 1 || a.n_workers >= 1 << 13 || a.heads_kv >= 1 << 10 || n_seg >= 1 << 20) return cudaErrorInvalidValue;
+    if (a.n_workers < 1 || a.n_workers >= 1 << 14 || a.heads_kv >= 1 << 10 || n_seg >= 1 << 20) return cudaErrorInvalidValue;
     const size_t smem = static_cast<size_t>(a.batch + 1) * 8 + static_cast<size_t>(n_seg < kSegInSmem ? n_seg : kSegInSmem) * 8;
     if (smem > 40 * 1024) {  // above the default limit; set per device, cheap enough for so large a batch
         cudaError_t e = cudaFuncSetAttribute(step_build_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,

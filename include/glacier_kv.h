@@ -272,7 +272,8 @@ typedef struct gkv_step_io {
  *   - the step's context is c + n (0 tokens: skipped by the decode), and the split-KV work list is
  *     the one gkv_upload_step builds.
  * The tables stay the caller's: the step's launches read d_block_tables, which must not change
- * until they have run.  A request is left out of the step (slots -1, decode output untouched, table
+ * until they have run; gkv_rope_append, whose rows come from the host, is refused on such a step
+ * (gkv_mrope_append reads them on the device).  A request is left out of the step (slots -1, decode output untouched, table
  * and ctx_out as before, GKV_EDEVICE from the next gkv_sync) when a length is negative, c + n
  * exceeds table_stride * block_size, its pages need more than n_new_blocks ids or its rows more
  * than max_tokens; all of them are left out of the decode (alone) when heads_kv times the chunks of 8

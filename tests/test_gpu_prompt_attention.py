@@ -234,3 +234,59 @@ def test_many_prompts(cuda, dtype, batch):
     lens = rng.choice([0, 0, 1, 2, 7, 130, 257], batch).tolist()
     q, k, v, cu = _inputs(lens, 2, 1, 64, 64, dtype, seed=batch)
     _check(q, k, v, cu, 0.125)
+
+
+@pytest.mark.parametrize("dtype,d", [("bf16", 128), ("f16", 64), ("f32", 64)])
+def test_broadcast_keys_and_values(cuda, dtype, d):
+    """One key and value head given as several (a stride of 0), and one row of queries as all."""
+    q, k, v, cu = _inputs([150, 40], 4, 1, d, d, dtype, seed=12)
+    _check(q, k.expand(-1, 2, -1), v.expand(-1, 2, -1), cu, 0.1)
+    _check(q[:1].expand(q.shape[0], -1, -1), k, v, cu, 0.1)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_infinite_sinks(cuda, dtype):
+    """A sink of minus infinity is none; one of plus infinity takes all the weight."""
+    import torch
+
+    q, k, v, cu = _inputs([150, 1], 2, 1, 64, 64, dtype, seed=13)
+    out, lse = _run(q, k, v, cu, 0.125, sinks=torch.tensor([-math.inf, math.inf], device="cuda"))
+    plain, plain_lse = _run(q, k, v, cu, 0.125)
+    assert torch.equal(out[:, 0], plain[:, 0]) and torch.equal(lse[:, 0], plain_lse[:, 0])
+    assert bool((out[:, 1] == 0).all()) and bool((lse[:, 1] == math.inf).all())
+
+
+@pytest.mark.parametrize("dtype,d", [("bf16", 128), ("f16", 64), ("f32", 128)])
+def test_replayed_with_other_lengths(cuda, dtype, d):
+    """Captured once, replayed with other prompts in the same buffers; rows behind the last one stay."""
+    import torch
+
+    pool = G.PagedBlockPool(1, 1, 2, d, 16, dtype="bf16")
+    n, batch = 900, 5
+    q, k, v, _ = _inputs([n], 4, 2, d, d, dtype, seed=14)
+    cu = torch.zeros(batch + 1, dtype=torch.int32, device="cuda")
+    out, lse = torch.empty(n, 4, d, dtype=q.dtype, device="cuda"), torch.empty(n, 4, device="cuda")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    pool.prompt_attention(q, k, v, cu, out, 0.1, lse=lse, stream=s)
+    s.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        pool.prompt_attention(q, k, v, cu, out, 0.1, lse=lse, stream=s)
+    for lens in ([900, 0, 0, 0, 0], [1, 300, 2, 257, 5], [0, 0, 0, 0, 0], [128, 128, 129, 64, 400]):
+        c = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+        with torch.cuda.stream(s):
+            cu.copy_(torch.from_numpy(c))
+            out.fill_(7.0)
+            lse.fill_(7.0)
+            graph.replay()
+        s.synchronize()
+        pool.sync(s)
+        ref, rlse, size, most = prompt_reference(q, k, v, c.tolist(), 0.1)
+        tol, ltol = prompt_tolerance(ref, size, most, d, 900, q.dtype)
+        m = int(c[-1])
+        assert_within(out[:m], ref[:m], tol[:m], str(lens))
+        assert_within(lse[:m], rlse[:m], ltol + 2.0 ** -23 * rlse[:m].abs(), str(lens))
+        assert bool((out[m:] == 7.0).all()) and bool((lse[m:] == 7.0).all())
+    graph.reset()
+    pool.close()

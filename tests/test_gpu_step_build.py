@@ -257,3 +257,21 @@ def test_more_context_than_the_work_list_counts(cuda):
     pool.sync()
     assert bool((out == 0.0).all())
     pool.close()
+
+
+def test_rows_known_on_the_device_alone(cuda):
+    """gkv_rope_append takes its rows from the host: refused on a built step, and not behind the next upload."""
+    import torch
+
+    pool = G.PagedBlockPool(4, 1, 1, 64, 16)
+    pool.reserve_step(1, 2, 4, 1)
+    pool.set_static_step()
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    pool.build_step(G.StepBuffers(t([[0, -1]]), t([3]), t([1]), t([]), max_tokens=4))
+    q, k, v = (torch.zeros(2, 1, 64, device="cuda") for _ in range(3))
+    with pytest.raises(G.InvalidOperationError):
+        pool.rope_append(0, q, k, v, [3, 4], 1)
+    pool.upload_step(np.zeros((1, 1), np.int32), np.array([5], np.int32), np.array([3, 4], np.int64))
+    pool.rope_append(0, q, k, v, [3, 4], 1)
+    pool.sync()
+    pool.close()
