@@ -85,7 +85,10 @@ __device__ __forceinline__ void weights8(const float* w, float (&x)[8]) {
 template <typename T, typename KV, bool NORM>
 __global__ void __launch_bounds__(kThreads, 4) mrope_append_kernel(const ArenaGeom g, const __grid_constant__ MropeParams a, const int tokens) {
     pdl_launch_dependents();  // the decode that follows waits for this grid before reading q or the arena
-    __shared__ __align__(16) float2 turn[kMaxTokens * kMropeMaxPairs];  // (cos, sin) * mscale of each token's pairs
+    // (cos, sin) * mscale of each token's pairs: pair 8 l + 2 e + f at ((e * half / 8) + l) * 2 + f, so that the
+    // lanes of a row read neighbouring 16 bytes.  (In the pairs' own order the lanes are 64 bytes apart and
+    // four of them meet in a bank.)
+    __shared__ __align__(16) float2 turn[kMaxTokens * kMropeMaxPairs];
     __shared__ int64_t k_row[kMaxTokens], v_row[kMaxTokens];            // each token's row of head 0 in the arenas, -1: not stored
     const int n_tok = a.dyn_tok ? min(__ldg(a.dyn_tok), a.n_tok) : a.n_tok;
     const int t0 = blockIdx.x * tokens;
@@ -102,7 +105,7 @@ __global__ void __launch_bounds__(kThreads, 4) mrope_append_kernel(const ArenaGe
         const int pos = __ldg(a.positions + axis[j] * a.pos_stride + t0 + t);
         float s, c;
         rope_sincos_f64(static_cast<double>(pos) * static_cast<double>(inv_freq[j]), s, c);
-        turn[i] = make_float2(c * a.mscale, s * a.mscale);
+        turn[t * half + ((j >> 1 & 3) * (half >> 3) + (j >> 3)) * 2 + (j & 1)] = make_float2(c * a.mscale, s * a.mscale);
     }
     if (threadIdx.x < nt) {
         const int64_t s = __ldg(a.slots + t0 + threadIdx.x);
@@ -144,7 +147,7 @@ __global__ void __launch_bounds__(kThreads, 4) mrope_append_kernel(const ArenaGe
         int64_t at = static_cast<int64_t>(t0) * out_stride + h * d;
         KV* k_dst = static_cast<KV*>(g.k) + h * g.k_head_stride;
         const float k_inv = !is_q && g.k_inv ? __ldg(g.k_inv + a.layer * hk + h) : 1.f;
-        const float4* w4 = reinterpret_cast<const float4*>(turn + u);
+        const float4* w4 = reinterpret_cast<const float4*>(turn) + (u >> 3);
 #pragma unroll 1
         for (int t = 0; t < nt; ++t, src += ts, at += out_stride, w4 += half / 2) {
             float x[8], y[8];
@@ -180,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, 4) mrope_append_kernel(const ArenaGe
                 float c[8], s[8];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float4 w = w4[e];
+                    const float4 w = w4[e * (half >> 3)];
                     c[2 * e] = w.x, s[2 * e] = w.y, c[2 * e + 1] = w.z, s[2 * e + 1] = w.w;
                 }
                 if (neox) {
