@@ -165,7 +165,11 @@ struct StepWorkspace {
     const int64_t* d_slots = nullptr;
     bool uploaded = false;
     bool device_step = false;    // the step came from gkv_step_build
-    bool built = false;          // and no launch has followed it
+    bool built = false;          // and no launch has followed it on built_on, its stream
+    cudaStream_t built_on = nullptr;
+    void launched(cudaStream_t st) {
+        if (st == built_on) built = false;
+    }
     std::vector<int32_t> h_ctx;  // ctx_lens of the uploaded step
     WorkList wl;                 // the uploaded step's work list (kept for its capacity)
     // chunked prefill: pinned + device buffer of its work items / work list, and q in the

@@ -634,6 +634,7 @@ int step_build(Pool* p, const gkv_step_io* io, int32_t batch, cudaStream_t st) {
     ws.up_max_blocks = io->table_stride;
     ws.uploaded = true;
     ws.built = ws.device_step = true;
+    ws.built_on = st;
     return GKV_OK;
 }
 
@@ -674,7 +675,7 @@ int step_append(Pool* p, int32_t layer, const float* d_k, const float* d_v, int3
                                      static_cast<int64_t>(p->desc.heads_kv) * p->desc.v_head_dim,
                                      ws.d_slots, 0, ws.static_mode ? ws.max_tokens : n_tok, ws.d_err, st, dyn_tok);
     if (e != cudaSuccess) return cuda_fail(e, "kv_append launch");
-    ws.built = false;
+    ws.launched(st);
     p->last_launches += 1;
     return GKV_OK;
 }
@@ -733,7 +734,7 @@ static int decode_common(Pool* p, int32_t layer, const float* d_q, float* d_out,
         // kernel that builds the header, an ordinary launch has to come between
         cudaError_t e = launch_order(st);
         if (e != cudaSuccess) return cuda_fail(e, "step order launch");
-        ws.built = false;
+        ws.launched(st);
         ++p->last_launches;
     }
     cudaError_t e = launch_paged_decode(p->geom, ws.work, a, &launches, st);
@@ -1092,7 +1093,7 @@ int step_rope_append(Pool* p, int32_t layer, float* d_q, const float* d_k, const
     a.err = ws.d_err;
     cudaError_t e = launch_rope_append(p->geom, a, st);
     if (e != cudaSuccess) return cuda_fail(e, "rope_append launch");
-    ws.built = false;
+    ws.launched(st);
     p->last_launches += 1;
     return GKV_OK;
 }
@@ -1212,7 +1213,7 @@ int step_mrope_append(Pool* p, int32_t layer, const gkv_qkv_io* io, int32_t n_to
     if (a.n_tok == 0) return GKV_OK;
     cudaError_t e = launch_mrope_append(p->geom, a, st);
     if (e != cudaSuccess) return cuda_fail(e, "mrope_append launch");
-    ws.built = false;
+    ws.launched(st);
     p->last_launches += 1;
     return GKV_OK;
 }
@@ -1268,7 +1269,7 @@ int step_prompt(Pool* p, const gkv_prompt_desc* r, cudaStream_t st) {
     cudaError_t e = launch_prompt_tc(a, &ran, st);
     if (e == cudaSuccess && !ran) e = launch_prompt_simt(a, st);
     if (e != cudaSuccess) return cuda_fail(e, "prompt_attention launch");
-    ws.built = false;
+    ws.launched(st);
     p->last_launches += 1;
     return GKV_OK;
 }

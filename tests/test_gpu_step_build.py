@@ -275,3 +275,29 @@ def test_rows_known_on_the_device_alone(cuda):
     pool.rope_append(0, q, k, v, [3, 4], 1)
     pool.sync()
     pool.close()
+
+
+def test_a_launch_on_another_stream_orders_nothing(cuda):
+    """Behind a build the decode waits for all of it, unless a launch on the build's own stream stands between."""
+    import torch
+
+    pool = G.PagedBlockPool(4, 1, 1, 64, 16)
+    pool.reserve_step(1, 2, 4, 1)
+    pool.set_static_step()
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    io = G.StepBuffers(t([[0, -1]]), t([3]), t([1]), t([]), max_tokens=4)
+    x = torch.zeros(4, 1, 64, device="cuda")
+    q, out = torch.zeros(1, 1, 64, device="cuda"), torch.zeros(1, 1, 64, device="cuda")
+    cu, one, two = t([0, 4]), torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    counts = []
+    for between in (None, two, one):
+        pool.build_step(io, stream=one.cuda_stream)
+        if between is not None:
+            pool.prompt_attention(x, x, x, cu, torch.empty_like(x), 1.0, stream=between.cuda_stream)
+        pool.paged_decode(0, q, out, 1, 1.0, stream=one.cuda_stream)
+        counts.append(pool.last_launch_count)
+        torch.cuda.synchronize()
+    pool.sync()
+    assert counts[0] == counts[1] == counts[2] + 1
+    pool.close()
