@@ -30,6 +30,13 @@
 // a not-finite value get it back in the epilogue.
 // Every wait is bounded: on expiry the block raises kErrWaitTimeout, lets its copies and products
 // finish, frees its tensor memory and ends.
+//
+// Measured (28 q and 4 kv heads of 128, bf16): 16384 tokens 1.38 ms = 1394 TFLOP/s, 83 % of the measured
+// product rate, and 1.6 ms where the card holds its power limit; tensor pipe and exponentials are each busy for
+// 71 % of the time.  24 prompts of 1 to 6000 tokens: 0.53 ms = 1100 TFLOP/s, first and last key tiles.  16 q
+// and 4 kv heads of 64 in fp16, 9 prompts of up to 4000 tokens: 0.137 ms = 590 TFLOP/s; with half the
+// products for the same exponentials those are the bound (0.068 ms), and short items leave the chain of
+// scores, softmax and P V bare.
 #include <cuda.h>
 
 #include <atomic>

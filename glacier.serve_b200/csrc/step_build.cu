@@ -21,6 +21,10 @@
 // Latency-bound: the bytes are a few per request and 12 per token.  So there is one launch and no
 // wait between its blocks: each block repeats the scan over the requests (at most 4096, from L2), the
 // first few plan, the others write tables, slots and positions.
+//
+// Measured, replayed in a graph: 64 decodes of 4 kv heads 6.5 us, 1024 decodes 9.0 us, 40 prompts of
+// together 48,000 tokens 6.5 us.  It is the chain of scan, cuts and numbering: with 64-bit products, binary
+// searches and five barriers a scan it took 16 to 24 us.
 #include "gkv_device.cuh"
 #include "kernels.h"
 #include "../../include/glacier_kv.h"
