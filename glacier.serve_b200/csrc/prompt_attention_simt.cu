@@ -11,9 +11,10 @@
 // 32-bit keys and values are copied asynchronously: values while the scores are formed, the next keys
 // while they are used.
 //
-// Measured (32 q and 8 kv heads of 128, 32 bits): 4 prompts of 4096 tokens 44 TFLOP/s, 59 % of the FMA rate of
-// 74.5; 6 ragged prompts of 90 to 1500 tokens 0.74 ms = 34.7 TFLOP/s, where the last tiles run alone.  The
-// FMA pipe is busy for two thirds of the time; one block of 8 warps an SM (184 KB) hides the rest no further.
+// Measured (32 q and 8 kv heads of 128, 32 bits): 4 prompts of 4096 tokens 45 TFLOP/s, 60 % of the FMA rate of
+// 74.5; 6 ragged prompts of 1 to 1500 tokens 0.70 ms = 36.5 TFLOP/s.  A key tile takes 13.5 us where its FMAs take
+// 8.3: shared memory gives 128 bytes a cycle to the registers, which the values (4 FMA a float) just live on
+// and the scores (8 / 3 FMA a float) do not, and one block of 8 warps an SM (184 KB) hides little of the softmax.
 #include "gkv_device.cuh"
 #include "kernels.h"
 #include "prompt_tiles.cuh"
@@ -117,12 +118,15 @@ __global__ void __launch_bounds__(kThreads) prompt_simt_kernel(const PromptArgs 
         copies_done();
         __syncthreads();  // the keys are there, and the last tile's values and weights have been used
         fill<kN, D>(sV, V + k0 * a.v_ts, a.v_ts, nk, a.dv);
+        // keys of the tile that a row of this warp sees (a multiple of 2 R): the products with the others are left out
+        const int seen = min(kN, q0 + ((ti & ~1) + 2) * R - k0);
         float2 s2[R][4];
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int c = 0; c < 4; ++c) s2[r][c] = make_float2(0.f, 0.f);
-#pragma unroll 4
+        if (seen > 0)
+#pragma unroll 2
         for (int e = 0; e < D; e += 4) {
             float4 kv[4];
 #pragma unroll
@@ -183,7 +187,7 @@ __global__ void __launch_bounds__(kThreads) prompt_simt_kernel(const PromptArgs 
         }
         if (finite) {
 #pragma unroll 1
-            for (int n = 0; n < kN; n += 4) {
+            for (int n = 0; n < seen; n += 4) {
                 float4 p[R];
 #pragma unroll
                 for (int r = 0; r < R; ++r) p[r] = *reinterpret_cast<const float4*>(sP + (ti * R + r) * LP + n);
