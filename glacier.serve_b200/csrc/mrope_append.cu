@@ -7,17 +7,17 @@
 // then rounded: at position 10^6 a product in 32 bits is off by up to 2^-5 rad.  Everything else is
 // 32 bits, rounded once to each destination's type.
 //
-// Roofline: HBM for prompts, launch latency for single tokens.  A block takes a few tokens (one
+// Roofline: HBM for prompts, launch latency for single tokens.  A block takes up to 16 tokens (one
 // where there are few), puts their cos and sin into shared memory once for all heads, and hands
 // each group of head_dim / 16 lanes one head row: a lane holds 8 pairs, read as two vectors of 8
 // elements (pairs (i, i + R/2)) or one of 16 (pairs (2i, 2i + 1)), so partners meet in a lane and
 // the norm's sum crosses lanes only log2(head_dim / 16) times.
 //
-// Measured (28 q and 4 kv heads of 128, 16 bits): 64 tokens 3.8 us; 8192 tokens with biases 39.7 us =
-// 4.2 TB/s, 65 % of the measured copy rate; 2049 tokens of 32 q and 8 kv heads with norms, 32 bits into an
+// Measured (28 q and 4 kv heads of 128, 16 bits): 64 tokens 3.8 us; 8192 tokens with biases 35.7 us =
+// 4.7 TB/s, 72 % of the measured copy rate; 2049 tokens of 32 q and 8 kv heads with norms, 32 bits into an
 // 8-bit arena, 21 us = 4.1 TB/s (513 blocks, one wave of 592).  What is left is latency: 47 % of the issue
-// slots are used and the warps wait for their rows.  Blocks of 3 or 6 tokens, 3 or 5 blocks an SM, rows
-// prefetched into registers and rows staged in shared memory were all slower.
+// slots are used and the warps wait for their rows.  3 or 5 blocks an SM, rows prefetched into registers and
+// rows staged in shared memory were all slower.
 #include "gkv_device.cuh"
 #include "kernels.h"
 #include "rope_math.cuh"
@@ -28,7 +28,12 @@ namespace gkv {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxTokens = 4;  // tokens per block
+constexpr int kMaxTokens = 16;    // tokens per block
+constexpr int kPlaces = 148 * 4;  // blocks that the card holds at a time
+// Blocks come in as few waves as kMaxTokens tokens each allow, and then take no more tokens than fill those: a
+// block's cos and sin and the loads of its bias cost once a block.  (4 a block for 8192 tokens: 39.2 instead of 35.7 us.)
+__host__ __device__ constexpr int block_waves(int n_tok) { return (n_tok - 1) / (kPlaces * kMaxTokens) + 1; }
+__host__ __device__ constexpr int block_tokens(int n_tok) { return (n_tok - 1) / (kPlaces * block_waves(n_tok)) + 1; }
 
 __device__ __forceinline__ float2 unpack(uint32_t w, __nv_bfloat16) {
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
@@ -89,17 +94,21 @@ __device__ __forceinline__ void weights8(const float* w, float (&x)[8]) {
 // T: the type of q, k and v; KV: the arena's; NORM: q or k has a norm weight.  Bound by issued
 // instructions as much as by memory: what does not depend on the token is computed once per head row.
 template <typename T, typename KV, bool NORM>
-__global__ void __launch_bounds__(kThreads, 4) mrope_append_kernel(const ArenaGeom g, const __grid_constant__ MropeParams a, const int tokens) {
+__global__ void __launch_bounds__(kThreads, 4) mrope_append_kernel(const ArenaGeom g, const __grid_constant__ MropeParams a, int tokens) {
     pdl_launch_dependents();  // the decode that follows waits for this grid before reading q or the arena
     // (cos, sin) * mscale of each token's pairs: pair 8 l + 2 e + f at ((e * half / 8) + l) * 2 + f, so that the
     // lanes of a row read neighbouring 16 bytes.  (In the pairs' own order the lanes are 64 bytes apart and
     // four of them meet in a bank.)
     __shared__ __align__(16) float2 turn[kMaxTokens * kMropeMaxPairs];
     __shared__ int64_t k_row[kMaxTokens], v_row[kMaxTokens];            // each token's row of head 0 in the arenas, -1: not stored
-    const int n_tok = a.dyn_tok ? min(__ldg(a.dyn_tok), a.n_tok) : a.n_tok;
+    int n_tok = a.n_tok;
+    if (a.dyn_tok) {  // the rows that are there decide, not those reserved
+        n_tok = min(__ldg(a.dyn_tok), n_tok);
+        tokens = block_tokens(n_tok);
+    }
+    if (static_cast<int64_t>(blockIdx.x) * tokens >= n_tok) return;
     const int t0 = blockIdx.x * tokens;
     const int nt = min(tokens, n_tok - t0);
-    if (nt <= 0) return;
     const int half = a.rope_dim / 2;
     // The tables are in the parameters, but are read as memory: 32 different addresses of the constant
     // bank are 32 reads one after the other.
@@ -243,9 +252,12 @@ __global__ void __launch_bounds__(kThreads, 4) mrope_append_kernel(const ArenaGe
 
 template <typename T, typename KV>
 cudaError_t launch_typed(const ArenaGeom& g, const MropeParams& p, cudaStream_t st) {
-    // one token per block until the card is full
-    const int tokens = p.n_tok <= 148 * 8 ? 1 : kMaxTokens;
-    const unsigned blocks = static_cast<unsigned>((static_cast<int64_t>(p.n_tok) + tokens - 1) / tokens);
+    const int tokens = block_tokens(p.n_tok);
+    unsigned blocks = static_cast<unsigned>((p.n_tok - 1) / tokens) + 1;
+    if (p.dyn_tok) {  // enough for any smaller count
+        const int64_t places = static_cast<int64_t>(kPlaces) * block_waves(p.n_tok);
+        blocks = static_cast<unsigned>(p.n_tok < places ? p.n_tok : places);
+    }
     if (p.q_norm || p.k_norm) mrope_append_kernel<T, KV, true><<<blocks, kThreads, 0, st>>>(g, p, tokens);
     else mrope_append_kernel<T, KV, false><<<blocks, kThreads, 0, st>>>(g, p, tokens);
     return cudaGetLastError();

@@ -223,3 +223,39 @@ def test_refusals(cuda):
         other.mrope_append(0, *x, pos, G.MultiAxisRope([24, 12, 12], 96), torch.empty_like(x[0]))
     pool.close()
     other.close()
+
+
+@pytest.mark.parametrize("static", [False, True])
+@pytest.mark.parametrize("n", [592, 593, 2049, 9472, 9473, 20001])
+def test_tokens_of_a_block(cuda, n, static):
+    """Counts around those that change how many tokens a block takes; in the static layout fewer rows than reserved."""
+    import torch
+
+    rng = np.random.default_rng(n)
+    g = torch.Generator(device="cuda").manual_seed(n)
+    heads, heads_kv, d, cap = 3, 1, 32, n + 9000 if static else n
+    blocks = -(-n // 16)
+    pool = G.PagedBlockPool(blocks, 1, heads_kv, d, 16, dtype="f32")
+    slots = _slots(rng, n, blocks, 16)
+    if static:
+        pool.reserve_step(1, 1, cap, heads)
+        pool.set_static_step()
+    pool.upload_step(np.zeros((1, 1), np.int32), np.ones(1, np.int32), slots)
+    q, k, v = (torch.randn(cap, h, d, device="cuda", generator=g) for h in (heads, heads_kv, heads_kv))
+    bias = torch.randn(heads * d, device="cuda", generator=g)
+    norm = 1 + 0.1 * torch.randn(d, device="cuda", generator=g)
+    rope = G.MultiAxisRope([8, 8], d)
+    pos = torch.tensor(rng.integers(0, 100_000, (2, cap)), dtype=torch.int32, device="cuda")
+    q_out = torch.full_like(q, 9.0)
+    pool.mrope_append(0, q, k, v, pos, rope, q_out, q_bias=bias, q_norm=norm)
+    pool.sync()
+    args = (pos[:, :n], rope.axis, rope.inv_freq, 0, 1.0)
+    ref, size = rope_reference(q[:n], *args, bias=bias, weight=norm)
+    assert_within(q_out[:n], ref, rope_tolerance(ref, size, d, q.dtype), "q")
+    assert bool((q_out[n:] == 9.0).all())
+    ref, size = rope_reference(k[:n], *args)
+    at = torch.tensor(slots, device="cuda")
+    keys, values = (x[:, 0, 0].reshape(-1, d)[at] for x in (pool.key_view(), pool.value_view()))
+    assert_within(keys[:, None], ref, rope_tolerance(ref, size, d, q.dtype), "k")
+    assert torch.equal(values, v[:n, 0])
+    pool.close()
