@@ -71,21 +71,24 @@ __device__ __forceinline__ void sort_prompts(const PromptArgs& a, PromptList& l,
     }
     if (thread == 0) l.sorted[a.batch] = 0;
 }
-// By one warp; returns the number of tiles.
+// By one warp; returns the number of tiles.  Sums stop at kTileLimit, above every tile number of a grid: prompts
+// that overlap (each range good by itself, the order of the rows not) may have more tiles than 32 bits count.
+constexpr int kTileLimit = 1 << 26;
 __device__ __forceinline__ int sum_prompt_levels(const PromptArgs& a, PromptList& l) {
     const int lane = threadIdx.x & 31;
     int sum = 0;
     for (int base = 0; base < a.batch; base += 32) {
         const int k = base + lane;
-        const int n = k < a.batch ? (k + 1) * (l.sorted[k] - l.sorted[k + 1]) : 0;
+        const int n = k < a.batch ? static_cast<int>(min(static_cast<int64_t>(k + 1) * (l.sorted[k] - l.sorted[k + 1]), int64_t{kTileLimit})) : 0;
         int inc = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int y = __shfl_up_sync(~0u, inc, o);
-            if (lane >= o) inc += y;
+            if (lane >= o) inc = min(inc + y, kTileLimit);
         }
-        if (k < a.batch) l.before[k] = sum + inc - n;
-        sum += __shfl_sync(~0u, inc, 31);
+        const int up = __shfl_up_sync(~0u, inc, 1);
+        if (k < a.batch) l.before[k] = min(sum + (lane ? up : 0), kTileLimit);
+        sum = min(sum + __shfl_sync(~0u, inc, 31), kTileLimit);
     }
     __syncwarp();
     return sum;

@@ -290,3 +290,21 @@ def test_replayed_with_other_lengths(cuda, dtype, d):
         assert bool((out[m:] == 7.0).all()) and bool((lse[m:] == 7.0).all())
     graph.reset()
     pool.close()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_overlapping_ranges_are_reported(cuda, dtype):
+    """More tiles than the rows of the call have: an error, and the next call is as any other."""
+    import torch
+
+    q, k, v, _ = _inputs([2000], 2, 1, 64, 64, dtype, seed=14)
+    pool = G.PagedBlockPool(1, 1, 1, 64, 16, dtype="f32")
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    first, then = torch.full_like(q, 7.0), torch.full_like(q, 7.0)
+    pool.prompt_attention(q, k, v, t([0, 2000] * 40), first, 0.125)
+    with pytest.raises(G.DeviceError):
+        pool.sync()
+    pool.prompt_attention(q, k, v, t([0, 2000]), then, 0.125)
+    pool.sync()
+    assert bool(((first == 7.0) | (first == then)).all())
+    pool.close()
