@@ -13,7 +13,7 @@
 // elements (pairs (i, i + R/2)) or one of 16 (pairs (2i, 2i + 1)), so partners meet in a lane and
 // the norm's sum crosses lanes only log2(head_dim / 16) times.
 //
-// Measured (28 q and 4 kv heads of 128, 16 bits): 64 tokens 3.8 us; 8192 tokens with biases 35.7 us =
+// Measured (28 q and 4 kv heads of 128, 16 bits): 64 tokens 3.9 us; 8192 tokens with biases 35.7 us =
 // 4.7 TB/s, 72 % of the measured copy rate; 2049 tokens of 32 q and 8 kv heads with norms, 32 bits into an
 // 8-bit arena, 21 us = 4.1 TB/s (513 blocks, one wave of 592).  What is left is latency: 47 % of the issue
 // slots are used and the warps wait for their rows.  3 or 5 blocks an SM, rows prefetched into registers and
