@@ -156,10 +156,17 @@ __device__ __forceinline__ int stolen_block(const uint32_t* response) {
     return ok ? static_cast<int>(x) : -1;
 }
 
-__device__ __forceinline__ void store_sector(void* p, const uint32_t (&w)[8]) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
-                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                 : "memory");
+// 32 bytes; `whole`: p is on a 32-byte boundary, which the one wide store needs (16 bytes do for the two).
+__device__ __forceinline__ void store_sector(void* p, const uint32_t (&w)[8], bool whole) {
+    if (whole) {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                     "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                     : "memory");
+    } else {
+        asm volatile("st.global.v4.b32 [%0], {%1, %2, %3, %4};\n\tst.global.v4.b32 [%0 + 16], {%5, %6, %7, %8};" ::"l"(p), "r"(w[0]),
+                     "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                     : "memory");
+    }
 }
 
 template <bool F16>
@@ -668,7 +675,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int rows = min(kBM, it.len - it.q0 - t * kBM);
             const int64_t row = it.row0 + it.q0 + t * kBM;
             if (a.lse && r < rows) a.lse[(row + r) * a.n_heads + it.head] = (top + log2f(total)) * 0.6931471805599453f;
-            // each row from its thread, in whole 32-byte sectors
+            // each row from its thread, in whole 32-byte sectors (rows are 128 or 256 bytes and dense, so the base decides)
+            const bool whole = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
             uint8_t* out = static_cast<uint8_t*>(a.out) + ((row + r) * a.n_heads + it.head) * (D * 2);
 #pragma unroll 1
             for (int h = 0; h < D / 64; ++h) {
@@ -682,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
                         w[e] = pack_16x2<F16>(__uint_as_float(o[c >> 5][(c & 31) + 2 * e]) * inv, __uint_as_float(o[c >> 5][(c & 31) + 2 * e + 1]) * inv);
-                    if (r < rows) store_sector(out + h * 128 + c * 2, w);
+                    if (r < rows) store_sector(out + h * 128 + c * 2, w, whole);
                 }
             }
             const volatile int* tags = bk->poisoned[it.number & 1];

@@ -1,0 +1,49 @@
+"""gkv_prompt_attention at the edges of what its documentation allows: alignment."""
+import math
+
+import pytest
+
+import glacier_kv as G
+from operator_refs import assert_within, prompt_reference, prompt_tolerance
+from test_gpu_prompt_attention import _inputs, _kind
+
+pytestmark = pytest.mark.gpu
+
+
+def _at(offset, shape, dtype, mark):
+    """(buffer, dense tensor of `shape` that starts `offset` elements into it, with room behind)."""
+    import torch
+
+    n = math.prod(shape)
+    buf = torch.full((offset + n + 64,), mark, dtype=dtype, device="cuda")
+    return buf, buf[offset:offset + n].view(shape)
+
+
+@pytest.mark.parametrize("dtype,d", [("bf16", 128), ("f16", 128), ("bf16", 64), ("f16", 64), ("f32", 128), ("bf16", 96)])
+@pytest.mark.parametrize("sixteens", [0, 1, 2, 3])
+def test_rows_on_any_16_byte_boundary(cuda, dtype, d, sixteens):
+    """q, k, v and out at every 16-byte boundary, lse at odd floats: nothing beside the rows is written."""
+    import torch
+
+    kind, h, hk = _kind(dtype), 4, 2
+    off = sixteens * 16 // torch.empty(0, dtype=kind).element_size()
+    q, k, v, cu = _inputs([200, 3, 129], h, hk, d, d, dtype, seed=21)
+    n = q.shape[0]
+    moved = []
+    for x in (q, k, v):
+        _, y = _at(off, x.shape, kind, 0.0)
+        y.copy_(x)
+        moved.append(y)
+    buf, out = _at(off, (n, h, d), kind, 7.0)
+    lbuf, lse = _at(sixteens, (n, h), torch.float32, 7.0)
+    assert out.data_ptr() % 16 == 0 and out.data_ptr() % 64 == 16 * sixteens
+    pool = G.PagedBlockPool(1, 1, hk, d, 16)
+    pool.prompt_attention(*moved, torch.tensor(cu, device="cuda"), out, 1 / math.sqrt(d), lse=lse)
+    pool.sync()
+    pool.close()
+    ref, rlse, size, most = prompt_reference(q, k, v, [int(c) for c in cu], 1 / math.sqrt(d))
+    tol, ltol = prompt_tolerance(ref, size, most, d, 200, kind)
+    assert_within(out, ref, tol, "out")
+    assert_within(lse, rlse, ltol + 2.0 ** -23 * rlse.abs(), "lse")
+    for b, o, m in ((buf, off, out.numel()), (lbuf, sixteens, lse.numel())):
+        assert bool((b[:o] == 7.0).all()) and bool((b[o + m:] == 7.0).all())
