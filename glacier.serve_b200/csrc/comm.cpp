@@ -343,12 +343,14 @@ int gkv_paged_decode_splitkv_dist(gkv_pool* pool, gkv_comm* c, int32_t layer, co
     float* send_lse = send_out + rows * dv;
     P.last_launches = 0;
     // rows this rank holds no tokens of keep lse = -inf (weight 0 in the merge); when every
-    // sequence has tokens here the decode writes every row and the fill launch is skipped
+    // sequence has tokens here the decode writes every row and the fill launch is skipped.  The
+    // contexts of a step built on the device are known there alone: it is always filled.
     cudaError_t e = cudaSuccess;
     int fills = 0;
-    if (std::find(P.ws.h_ctx.begin(), P.ws.h_ctx.end(), 0) != P.ws.h_ctx.end()) {
+    if (P.ws.device_step || std::find(P.ws.h_ctx.begin(), P.ws.h_ctx.end(), 0) != P.ws.h_ctx.end()) {
         e = gkv::launch_fill(send_lse, rows, -INFINITY, st);
         if (e != cudaSuccess) return gkv::cuda_fail(e, "fill launch");
+        P.ws.launched(st);
         fills = 1;
     }
     int rc = gkv::step_decode_lse(&P, layer, d_q, send_out, send_lse, n_heads, scale, nullptr, st);

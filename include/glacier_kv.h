@@ -577,7 +577,8 @@ GKV_API int gkv_comm_exchange_kind(const gkv_comm* comm);
  * mailbox, one kernel publishes an epoch flag, waits for every rank's and merges), else an NCCL
  * all-gather -- and the log-sum-exp merge (plus the optional sinks, applied once) into d_out
  * [batch][n_heads][v_head_dim] on every rank.  All ranks must call it with the same batch and
- * n_heads.  Merged rows of sequences with no tokens on any rank are 0. */
+ * n_heads.  Merged rows of sequences with no tokens on any rank are 0, behind gkv_step_build too
+ * (requests that it left out have none). */
 GKV_API int gkv_paged_decode_splitkv_dist(gkv_pool* pool, gkv_comm* comm, int32_t layer,
                                           const float* d_q, float* d_out, int32_t n_heads,
                                           float scale, const float* d_sinks, void* stream);
