@@ -61,6 +61,9 @@ constexpr uint32_t kTmemCols = 512;               // S0 S1 O0 O1, 128 columns ea
 constexpr uint32_t kColS = 0, kColO = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleLog2 = 8.f;
+// The running maximum starts at the type's lowest value: against minus infinity a row whose scores so far are all
+// minus infinity would have weights of 2^(-inf + inf), NaN for good; against this they are 0, as they should be.
+constexpr float kLowest = -3.402823466e+38f;
 constexpr uint32_t kPolls = 1u << 24;
 constexpr uint32_t kPlanNs = 100, kLoadNs = 40, kMmaNs = 0, kSoftNs = 0;
 
@@ -641,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int n = t ? it.n[1] : it.n[0];
             const int nj = it.n[1] ? it.n[1] : it.n[0];
             const int pos = it.q0 + t * kBM + r;
-            float m_run = -INFINITY, l_run = 0.f;
+            float m_run = kLowest, l_run = 0.f;
             for (int j = 0; j < n; ++j) {
                 if (j == n - 1) {  // while the scores are on their way
                     const uint32_t vs = slot0 + 2 * j + 1;
@@ -665,9 +668,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (a.sinks) {
                 const float sink = __ldg(a.sinks + it.head) * kLog2e;
                 top = fmaxf(m_run, sink);
-                const float base = top == -INFINITY ? 0.f : top;
-                const float alpha = fast_exp2(m_run - base);
-                total = l_run * alpha + (sink == base ? 1.f : fast_exp2(sink - base));  // also where both are infinite
+                const float alpha = fast_exp2(m_run - top);
+                total = l_run * alpha + (sink == top ? 1.f : fast_exp2(sink - top));  // also where both are infinite
                 inv = alpha / total;
             } else {
                 inv = 1.f / l_run;

@@ -1,4 +1,4 @@
-"""gkv_prompt_attention at the edges of what its documentation allows: alignment."""
+"""gkv_prompt_attention at the edges of what its documentation allows: alignment, scores of minus infinity."""
 import math
 
 import pytest
@@ -47,3 +47,32 @@ def test_rows_on_any_16_byte_boundary(cuda, dtype, d, sixteens):
     assert_within(lse, rlse, ltol + 2.0 ** -23 * rlse.abs(), "lse")
     for b, o, m in ((buf, off, out.numel()), (lbuf, sixteens, lse.numel())):
         assert bool((b[:o] == 7.0).all()) and bool((b[o + m:] == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype,d", [("bf16", 128), ("f16", 64), ("f32", 64)])
+@pytest.mark.parametrize("cut", [1, 127, 128, 200, 256, 300, 511])
+@pytest.mark.parametrize("sink", [None, -3.0])
+def test_first_keys_score_minus_infinity(cuda, dtype, d, cut, sink):
+    """Keys that score -infinity weigh nothing: rows behind them are as if they were not there, and a row that sees no
+    other key has 0 / 0, or, with a sink, all its weight there."""
+    import torch
+
+    n, h, hk = 600, 4, 2
+    q, k, v, _ = _inputs([n], h, hk, d, d, dtype, seed=22)
+    q[..., 0] = q[..., 0].abs() + 1
+    k[:cut, :, 0] = -math.inf
+    sinks = None if sink is None else torch.full((h,), sink, device="cuda")
+    pool = G.PagedBlockPool(1, 1, hk, d, 16)
+    out, lse = torch.empty_like(q), torch.empty(n, h, device="cuda")
+    pool.prompt_attention(q, k, v, torch.tensor([0, n], dtype=torch.int32, device="cuda"), out, 1 / math.sqrt(d), sinks=sinks, lse=lse)
+    pool.sync()
+    pool.close()
+    ref, rlse, size, most = prompt_reference(q[cut:], k[cut:], v[cut:], [0, n - cut], 1 / math.sqrt(d), sinks)
+    tol, ltol = prompt_tolerance(ref, size, most, d, n, q.dtype)
+    assert_within(out[cut:], ref, tol, "rows behind")
+    assert_within(lse[cut:], rlse, ltol + 2.0 ** -23 * rlse.abs(), "lse behind")
+    if sink is None:
+        assert bool(out[:cut].isnan().all()) and bool((lse[:cut] == -math.inf).all())
+    else:
+        assert bool((out[:cut] == 0).all())
+        assert_within(lse[:cut], torch.full((cut, h), sink, dtype=torch.float64, device="cuda"), torch.tensor(2.0 ** -21 * abs(sink), device="cuda"), "lse")
