@@ -17,7 +17,33 @@ struct PromptTile {
 // One more than the largest tile number.
 inline int64_t prompt_tile_bound(const PromptArgs& a, int tile_rows) { return a.total / tile_rows + a.batch; }
 
-// Every thread of a warp calls it with the same x; false where no tile has that number.
+// Tiles of a prompt, none where its range is bad.
+template <int T>
+__device__ __forceinline__ int tiles_of(int begin, int end, int total) {
+    return begin >= 0 && end >= begin && end <= total ? (end - begin) / T + ((end - begin) % T != 0) : 0;
+}
+
+// The prompt of tile number x by going over all of them: where bad ranges have led the search astray.
+template <int T>
+__device__ __noinline__ int prompt_of_tile(const int32_t* cu, int batch, int total, int x) {
+    const int lane = threadIdx.x & 31;
+    for (int base = 0; base < batch; base += 32) {
+        const int b = base + lane;
+        bool mine = false;
+        if (b < batch) {
+            const int begin = __ldg(cu + b), n = tiles_of<T>(begin, __ldg(cu + b + 1), total);
+            mine = n > 0 && x >= begin / T + b && x - (begin / T + b) < n;
+        }
+        const unsigned found = __ballot_sync(~0u, mine);
+        if (found) return base + __ffs(found) - 1;
+    }
+    return -1;
+}
+
+// Every thread of a warp calls it with the same x; false where no tile has that number.  The search is exact where
+// the ranges are good.  Next to a bad one (left out) it may end anywhere; but where it ends at a good prompt whose first
+// number and the next prompt's enclose x, x is this prompt's or nobody's: good prompts that follow one another
+// without overlap have their numbers in order.  Only otherwise are all prompts gone over.
 template <int T>
 __device__ __forceinline__ bool find_prompt_tile(const PromptArgs& a, int x, PromptTile& out) {
     const int lane = threadIdx.x & 31;
@@ -31,12 +57,17 @@ __device__ __forceinline__ bool find_prompt_tile(const PromptArgs& a, int x, Pro
         lo += at;
         n = min(step, n - at);
     }
-    const int begin = __ldg(a.cu + lo), end = __ldg(a.cu + lo + 1);
-    if (begin < 0 || end < begin || end > a.total) return false;
+    int begin = __ldg(a.cu + lo), end = __ldg(a.cu + lo + 1);
+    const bool good = begin >= 0 && end >= begin && end <= a.total;
+    if (!good || (lo > 0 && x < begin / T + lo) || (lo + 1 < a.batch && x > end / T + lo)) {
+        lo = prompt_of_tile<T>(a.cu, a.batch, a.total, x);
+        if (lo < 0) return false;
+        begin = __ldg(a.cu + lo), end = __ldg(a.cu + lo + 1);
+    }
     out.row0 = begin;
     out.len = end - begin;
     out.tile = x - (begin / T + lo);
-    return out.tile >= 0 && static_cast<int64_t>(out.tile) * T < out.len;
+    return out.tile >= 0 && out.tile < tiles_of<T>(begin, end, a.total);
 }
 
 // The tiles of up to kListed prompts in descending order of their keys: first every prompt's last tile
@@ -55,7 +86,7 @@ template <int T>
 __device__ __forceinline__ void count_prompt_tiles(const PromptArgs& a, PromptList& l, int thread, int threads) {
     for (int b = thread; b < a.batch; b += threads) {
         const int begin = __ldg(a.cu + b), end = __ldg(a.cu + b + 1);
-        l.count[b] = begin >= 0 && end >= begin && end <= a.total ? (end - begin) / T + ((end - begin) % T != 0) : 0;
+        l.count[b] = tiles_of<T>(begin, end, a.total);
     }
 }
 __device__ __forceinline__ void sort_prompts(const PromptArgs& a, PromptList& l, int thread, int threads) {

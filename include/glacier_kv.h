@@ -405,7 +405,8 @@ typedef struct gkv_prompt_desc {
  * before p . v), the others in 32-bit arithmetic; softmax statistics are 32 bits.  Masked keys and
  * values, and rows of other requests, never reach a result, whatever they hold.  Rows behind
  * cu_seqlens[batch] are left alone.  A prompt whose range is negative or passes `total` is left out
- * (GKV_EDEVICE from the next gkv_sync).  head_dim and v_head_dim must be multiples of 8 and at most
+ * (GKV_EDEVICE from the next gkv_sync); the others keep their results where their rows follow one
+ * another, and what two ranges share is either's.  head_dim and v_head_dim must be multiples of 8 and at most
  * 256 (GKV_EUNSUPPORTED); element strides and pointers must keep every head row 16-byte aligned
  * (GKV_EINVAL).  d_out and d_lse must not overlap the inputs.  Replaces, for a fresh prompt, the
  * per-token loop of PagedTransformerRunner.ForwardPrefillSubBatch (PagedTransformerRunner.cs:424-471). */

@@ -1,4 +1,4 @@
-"""gkv_prompt_attention at the edges of what its documentation allows: alignment, scores of minus infinity."""
+"""gkv_prompt_attention at the edges of what its documentation allows: alignment, scores of minus infinity, bad ranges."""
 import math
 
 import pytest
@@ -76,3 +76,62 @@ def test_first_keys_score_minus_infinity(cuda, dtype, d, cut, sink):
     else:
         assert bool((out[:cut] == 0).all())
         assert_within(lse[:cut], torch.full((cut, h), sink, dtype=torch.float64, device="cuda"), torch.tensor(2.0 ** -21 * abs(sink), device="cuda"), "lse")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("cu,served", [([0, 40, 30, 100], [(0, 0, 30), (30, 40, 100)]), ([-5, 40, 100], [(40, 40, 100)]),
+                                       ([0, 40, 101], [(0, 0, 40)]), ([0, 200, 60], [])])
+def test_good_prompts_beside_bad_ranges(cuda, dtype, cu, served):
+    """served: (first row of the prompt, first and last row that it alone holds); rows of bad ranges alone stay."""
+    import torch
+
+    q, k, v, _ = _inputs([100], 2, 1, 64, 64, dtype, seed=23)
+    out = torch.full_like(q, 7.0)
+    pool = G.PagedBlockPool(1, 1, 1, 64, 16)
+    pool.prompt_attention(q, k, v, torch.tensor(cu, dtype=torch.int32, device="cuda"), out, 0.125)
+    with pytest.raises(G.DeviceError):
+        pool.sync()
+    pool.sync()
+    pool.close()
+    free = torch.ones(100, dtype=torch.bool, device="cuda")
+    for first, b, e in served:
+        ref, _, size, most = prompt_reference(q, k, v, [first, e], 0.125)
+        tol, _ = prompt_tolerance(ref, size, most, 64, 100, q.dtype)
+        assert_within(out[b:e], ref[b:e], tol[b:e], str((first, b, e)))
+        free[first:e] = False
+    assert bool((out[free] == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("batch", [12, 70, 1030, 3000])
+@pytest.mark.parametrize("kind", ["past total", "negative", "first", "last", "several"])
+def test_good_prompts_beside_bad_ranges_of_large_batches(cuda, dtype, batch, kind):
+    """On both sides of what a block lists: the prompts whose ranges are good keep their results."""
+    import numpy as np
+    import torch
+
+    rng = np.random.default_rng(batch)
+    lens = rng.choice([1, 2, 7, 130, 257], batch).tolist()
+    q, k, v, cu = _inputs(lens, 2, 1, 64, 64, dtype, seed=24)
+    n = int(cu[-1])
+    bad = np.array(cu, np.int64)
+    at = {"first": [0], "last": [batch], "several": [batch // 5, batch // 2, batch // 2 + 1, 4 * batch // 5]}.get(kind, [batch // 2])
+    bad[at] = -1 if kind in ("negative", "first") else n + 100000
+    if kind == "several":
+        bad[at[1]] = -5
+    good = [b for b in range(batch) if 0 <= bad[b] <= bad[b + 1] <= n]
+    assert len(good) == batch - len({x for i in at for x in (i - 1, i) if 0 <= x < batch})
+    out = torch.full_like(q, 7.0)
+    pool = G.PagedBlockPool(1, 1, 1, 64, 16)
+    pool.prompt_attention(q, k, v, torch.tensor(bad, dtype=torch.int32, device="cuda"), out, 0.125)
+    with pytest.raises(G.DeviceError):
+        pool.sync()
+    want = torch.empty_like(q)
+    pool.prompt_attention(q, k, v, torch.tensor(cu, dtype=torch.int32, device="cuda"), want, 0.125)
+    pool.sync()
+    pool.close()
+    rows = torch.zeros(n, dtype=torch.bool, device="cuda")
+    for b in good:
+        rows[cu[b]:cu[b + 1]] = True
+    assert torch.equal(out[rows], want[rows])  # a tile's sums do not depend on where it runs
+    assert bool((out[~rows] == 7.0).all())
