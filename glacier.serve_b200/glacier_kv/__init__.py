@@ -408,7 +408,9 @@ class PagedBlockPool:
     def build_step(self, io: "StepBuffers", batch: Optional[int] = None, n_new_blocks: Optional[int] = None, stream=None) -> None:
         """gkv_step_build: block tables, slot mapping, positions and work list of a step from the
         request lengths in `io`, on the GPU (static step layout).  `batch` and `n_new_blocks`
-        default to the sizes of io's tensors."""
+        default to the sizes of io's tensors.  The tables' earlier entries are the caller's to keep: a
+        block that BlockTable.append_token forked (an offset other than 0 and an id other than the
+        entry's) is written into io.block_tables, and its copy flushed (flush_copies), before the build."""
         if io.device != self.device:
             raise ValueError(f"the step's arrays are on cuda:{io.device}, the pool on cuda:{self.device}")
         b = io.max_batch if batch is None else batch

@@ -266,7 +266,13 @@ typedef struct gkv_step_io {
  * Request b has c = ctx_lens[b] tokens stored and adds n = new_lens[b]:
  *   - pages ceil(c / block_size) .. ceil((c + n) / block_size) - 1 of its table take the next ids
  *     of new_blocks, requests in order (the host allocates them, e.g. by gkv_table_append_token);
- *     earlier entries are read, never written;
+ *     earlier entries are read, never written: the caller keeps them current.  Where
+ *     gkv_table_append_token forks a shared, partly filled last block (it returns an id other than
+ *     entry c / block_size, with an offset other than 0), that id belongs not into new_blocks but into
+ *     entry c / block_size of d_block_tables, before the build runs; otherwise the new tokens land in the
+ *     block that other requests still share.  Entries that gkv_pool_compact moves are rewritten the same way.
+ *     The copies that forks queue are issued on the stream first (gkv_pool_flush_copies; a replayed
+ *     build calls nothing that would);
  *   - its rows are cu_new[b] .. cu_new[b + 1] - 1 of the step, at positions c, c + 1, ... and the
  *     slots of their pages.  Entries of d_slots and d_positions behind the last row are left alone;
  *   - the step's context is c + n (0 tokens: skipped by the decode), and the split-KV work list is
