@@ -456,7 +456,7 @@ class PagedBlockPool:
                                     rope._desc, pro, _queue(stream, dev)))
 
     def prompt_attention(self, q, k, v, cu_seqlens, out, scale: float, sinks=None, lse=None, stream=None) -> None:
-        """Causal attention of packed whole prompts over their own k and v (gkv_prompt_attention):
+        """Causal attention of packed whole prompts over their own k and v, no tokens stored before (gkv_prompt_attention):
         q [total, n_heads, head_dim], k, v [total, heads_kv, ...] CUDA tensors of one type (float32,
         bfloat16, float16) with strides; cu_seqlens [batch + 1] int32 CUDA; out dense [total, n_heads,
         v_head_dim] of the same type; sinks [n_heads] and lse [total, n_heads] float32 CUDA or None."""

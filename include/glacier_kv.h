@@ -277,6 +277,12 @@ typedef struct gkv_step_io {
  *     slots of their pages.  Entries of d_slots and d_positions behind the last row are left alone;
  *   - the step's context is c + n (0 tokens: skipped by the decode), and the split-KV work list is
  *     the one gkv_upload_step builds.
+ * What attends the rows: gkv_paged_decode takes q and writes its output by REQUEST (row b of [batch]),
+ * over all c + n tokens, so its rows are the step's own only where every request adds one token; in a
+ * mixed step the caller gathers row cu_new[b + 1] - 1 of each request first.  gkv_prompt_attention over
+ * d_cu_new serves requests that had nothing stored (c = 0); of the others its rows attend the new
+ * tokens alone.  A further chunk (c > 0, n > 1) needs gkv_paged_prefill, behind gkv_upload_step in the
+ * ordinary layout: no call of the static layout attends it.
  * The tables stay the caller's: the step's launches read d_block_tables, which must not change
  * until they have run; gkv_rope_append, whose rows come from the host, is refused on such a step
  * (gkv_mrope_append reads them on the device).  A request is left out of the step (slots -1, decode output untouched, table
@@ -401,7 +407,7 @@ typedef struct gkv_prompt_desc {
     float scale;
 } gkv_prompt_desc;
 /* Causal attention of whole prompts over their own keys and values, read from the projections
- * (gkv_mrope_append's outputs) and not from the arena: row t of a request is
+ * (gkv_mrope_append's outputs) and not from the arena (tokens stored before are not seen): row t of a request is
  * softmax(scale * q_t . k_s [, sink]) . v_s over its rows s <= t, query head h reading kv head
  * h / (n_heads / heads_kv).  Beside gkv_paged_prefill, which reads the arena in its storage type
  * and lengths from the host, this one takes lengths on the device (d_cu_new of gkv_step_build),

@@ -120,3 +120,81 @@ def test_a_forked_block_is_rewritten_on_the_device(cuda, replayed):
     if replayed:
         graph.reset()
     pool.close()
+
+
+def _attended(pool, table, q, position, scale):
+    """(out, weighted |v|, largest sum of |q k|) in 64 bits of one query row [heads, dim] over the arena's positions 0 .. position."""
+    import torch
+
+    bs, at = pool.block_size, torch.arange(position + 1, device="cuda")
+    blocks = torch.tensor(table, device="cuda")[at // bs]
+    kk, vv = (x[blocks, 0, :, at % bs].double().repeat_interleave(q.shape[0] // x.shape[2], 1) for x in (pool.key_view(), pool.value_view()))
+    s = scale * torch.einsum("hd,thd->ht", q.double(), kk)
+    w = torch.softmax(s, 1)
+    most = float((abs(scale) * torch.einsum("hd,thd->ht", q.double().abs(), kk.abs())).max())
+    return torch.einsum("ht,thd->hd", w, vv), torch.einsum("ht,thd->hd", w, vv.abs()), most
+
+
+def test_prompts_and_tokens_in_one_step_then_a_further_chunk(cuda):
+    """The step's rows go to prompt attention as packed, to the decode gathered by request; a chunk behind stored tokens
+    goes through the ordinary layout."""
+    import numpy as np
+    import torch
+
+    from operator_refs import assert_within, prompt_reference, prompt_tolerance
+
+    g = torch.Generator(device="cuda").manual_seed(33)
+    H, HK, D, BS = 4, 2, 64, 16
+    scale = 1 / math.sqrt(D)
+    ctx, new = [40, 0, 15, 0, 16], [1, 37, 1, 1, 1]  # two prompts, one of them of a single token, and three tokens
+    B, cap, width = len(ctx), 48, 6
+    pool = G.PagedBlockPool(30, 1, HK, D, BS)
+    _random_arena(pool, g)
+    pool.reserve_step(B, width, cap, H)
+    pool.set_static_step()
+    tables = torch.full((B, width), -1, dtype=torch.int32, device="cuda")
+    ids = iter(torch.randperm(30, generator=torch.Generator().manual_seed(1)).tolist())
+    for b, c in enumerate(ctx):
+        for j in range(-(-c // BS)):
+            tables[b, j] = next(ids)
+    fresh = [next(ids) for c, n in zip(ctx, new) for _ in range(-(-(c + n) // BS) - -(-c // BS))]
+    io = G.StepBuffers(tables, _i32(ctx), _i32(new), _i32(fresh), max_tokens=cap)
+    rope = G.MultiAxisRope([D // 2], D)
+    q, k, v = (torch.randn(cap, n, D, device="cuda", generator=g) for n in (H, HK, HK))
+    q_out, k_out, out = torch.empty_like(q), torch.empty_like(k), torch.full_like(q, 7.0)
+    pool.build_step(io)
+    pool.mrope_append(0, q, k, v, io.positions[None], rope, q_out, k_out)
+    pool.prompt_attention(q_out, k_out, v, io.cu_new, out, scale)
+    tokens = torch.tensor([b for b, c in enumerate(ctx) if c > 0], device="cuda")
+    last = io.cu_new[1:].long() - 1
+    decoded = torch.empty(B, H, D, device="cuda")
+    pool.paged_decode(0, q_out[last].contiguous(), decoded, H, scale)
+    out[last[tokens]] = decoded[tokens]
+    pool.sync()
+    rows = io.block_tables.tolist()
+    cu = io.cu_new.tolist()
+    for b, (c, n) in enumerate(zip(ctx, new)):
+        if c == 0:
+            at = slice(cu[b], cu[b + 1])
+            ref, _, size, most = prompt_reference(q_out[at], k_out[at], v[at], [0, n], scale)
+            assert_within(out[at], ref, prompt_tolerance(ref, size, most, D, n, torch.float32)[0], f"prompt {b}")
+        else:
+            ref, size, most = _attended(pool, rows[b], q_out[cu[b]], c, scale)
+            assert_within(out[cu[b]], ref, prompt_tolerance(ref, size, most, D, c + 1, torch.float32)[0], f"token {b}")
+    assert bool((out[cu[-1]:] == 7.0).all())
+
+    # nine more tokens of request 1 (37 stored)
+    pool.set_static_step(False)
+    have, more = 37, 9
+    table = np.array([rows[1]], np.int32)
+    slots = np.array([rows[1][p // BS] * BS + p % BS for p in range(have, have + more)], np.int64)
+    pool.upload_step(table, np.array([have + more], np.int32), slots)
+    kn, vn, qn = (torch.randn(more, n, D, device="cuda", generator=g) for n in (HK, HK, H))
+    pool.kv_append(0, kn, vn)
+    chunk = torch.empty(more, H, D, device="cuda")
+    pool.paged_prefill(0, qn, chunk, [have], [more], H, scale)
+    pool.sync()
+    for i in range(more):
+        ref, size, most = _attended(pool, rows[1], qn[i], have + i, scale)
+        assert_within(chunk[i], ref, prompt_tolerance(ref, size, most, D, have + more, torch.float32)[0], f"chunk {i}")
+    pool.close()
