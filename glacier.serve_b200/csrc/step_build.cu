@@ -44,17 +44,16 @@ __device__ __forceinline__ uint32_t add_to_limit(uint32_t a, uint32_t b) { retur
 struct Counts {
     uint32_t rows, pages;  // at most 2^31 - 1 each
     uint32_t live;         // requests with units
-    uint32_t left;         // requests left out
     int64_t units;
     static __device__ __forceinline__ Counts plus(const Counts& a, const Counts& b) {
-        return Counts{add_to_limit(a.rows, b.rows), add_to_limit(a.pages, b.pages), a.live + b.live, a.left + b.left, a.units + b.units};
+        return Counts{add_to_limit(a.rows, b.rows), add_to_limit(a.pages, b.pages), a.live + b.live, a.units + b.units};
     }
     static __device__ __forceinline__ Counts up(const Counts& a, int o) {
         return Counts{__shfl_up_sync(~0u, a.rows, o), __shfl_up_sync(~0u, a.pages, o), __shfl_up_sync(~0u, a.live, o),
-                      __shfl_up_sync(~0u, a.left, o), __shfl_up_sync(~0u, a.units, o)};
+                      __shfl_up_sync(~0u, a.units, o)};
     }
     static __device__ __forceinline__ Counts at(const Counts& a, int l) {
-        return Counts{__shfl_sync(~0u, a.rows, l), __shfl_sync(~0u, a.pages, l), __shfl_sync(~0u, a.live, l), __shfl_sync(~0u, a.left, l),
+        return Counts{__shfl_sync(~0u, a.rows, l), __shfl_sync(~0u, a.pages, l), __shfl_sync(~0u, a.live, l),
                       __shfl_sync(~0u, a.units, l)};
     }
 };
@@ -337,13 +336,13 @@ __device__ __forceinline__ Counts scan_requests(const StepBuildArgs& a, Counts* 
         const bool counted = b < a.batch && r.fits;
         int64_t chunks = counted ? chunks_in(r.ctx + r.n, a.block_size) : 0;
         const Counts was = sum;
-        Counts at = block_scan(Counts{r.n, r.opened, chunks > 0, 0, chunks > 0 ? chunks + kSegmentCost : 0}, sum, part, turn);
+        Counts at = block_scan(Counts{r.n, r.opened, chunks > 0, chunks > 0 ? chunks + kSegmentCost : 0}, sum, part, turn);
         bool ok = counted;
         if (sum.rows > static_cast<uint32_t>(a.max_tokens) || sum.pages > static_cast<uint32_t>(a.n_new_blocks)) {  // the same for all threads
             ok = counted && served(a, r, at.rows, at.pages);
             if (!ok) chunks = 0;
             Counts again = was;
-            const Counts ua = block_scan(Counts{0, 0, chunks > 0, 0, chunks > 0 ? chunks + kSegmentCost : 0}, again, part, turn);
+            const Counts ua = block_scan(Counts{0, 0, chunks > 0, chunks > 0 ? chunks + kSegmentCost : 0}, again, part, turn);
             at.live = ua.live;
             at.units = ua.units;
             sum.live = again.live;
