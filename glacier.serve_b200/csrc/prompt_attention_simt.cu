@@ -25,8 +25,11 @@ namespace gkv {
 namespace {
 
 constexpr int kN = 64, kThreads = 256;
-// Batches up to which every block sorts the prompts for itself, to take the tiles with the most keys
-// first (2 us of some 20 to 300 a tile); the others go prompt by prompt.
+// Batches up to which every block sorts the prompts for itself, to take the tiles with the most keys first; the others
+// go prompt by prompt.  Here every tile of every head does that, so the limit is lower than kListed.  Sorted against
+// prompt by prompt, 28 heads and 4 heads, us: prompts of 1 to 2000 tokens (median 100) 64: 1723 / 1697 and 409 / 523,
+// 128: 1917 / 1846 and 290 / 326, 512: 15657 / 12203 and 2252 / 1818; prompts of 16 tokens 64: 237 / 224 and 39 / 37,
+// 512: 3302 / 1683 and 481 / 246.
 constexpr int kSorted = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 

@@ -103,7 +103,7 @@ def test_good_prompts_beside_bad_ranges(cuda, dtype, cu, served):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
-@pytest.mark.parametrize("batch", [12, 70, 1030, 3000])
+@pytest.mark.parametrize("batch", [12, 64, 65, 512, 513, 1030, 3000])
 @pytest.mark.parametrize("kind", ["past total", "negative", "first", "last", "several"])
 def test_good_prompts_beside_bad_ranges_of_large_batches(cuda, dtype, batch, kind):
     """On both sides of what a block lists: the prompts whose ranges are good keep their results."""
@@ -135,3 +135,15 @@ def test_good_prompts_beside_bad_ranges_of_large_batches(cuda, dtype, batch, kin
         rows[cu[b]:cu[b + 1]] = True
     assert torch.equal(out[rows], want[rows])  # a tile's sums do not depend on where it runs
     assert bool((out[~rows] == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype,batch", [("bf16", 511), ("bf16", 512), ("bf16", 513), ("f16", 512), ("f32", 64), ("f32", 65)])
+def test_batches_around_the_listing_limits(cuda, dtype, batch):
+    """The most prompts that a block lists, and one more."""
+    import numpy as np
+
+    from test_gpu_prompt_attention import _check
+
+    lens = np.random.default_rng(batch).choice([0, 1, 3, 128, 130, 300], batch).tolist()
+    q, k, v, cu = _inputs(lens, 2, 1, 64, 64, dtype, seed=batch)
+    _check(q, k, v, cu, 0.125)
