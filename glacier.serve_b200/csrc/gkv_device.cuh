@@ -17,7 +17,7 @@ enum : int {
     kErrBadBlock = 1,      // a block id outside [0, total_blocks) reached a kernel
     kErrWaitTimeout = 2,   // a bounded mbarrier wait expired
     kErrBadSlot = 4,       // an append slot outside the arena
-    kErrBadStep = 8        // a request that a device-built step had to leave out
+    kErrBadStep = 8        // a request that a device-built step, or a prompt that its attention, had to leave out
 };
 
 // Upper bound of try_wait polls before a wait is declared stuck.  Each try_wait blocks for

@@ -1611,7 +1611,7 @@ int gkv_sync(gkv_pool* pool, void* stream, int32_t timeout_ms) {
             // a decode that stopped early may leave merge counters raised: start clean
             if (pool->impl.ws.d_merge_count)
                 cudaMemset(pool->impl.ws.d_merge_count, 0, pool->impl.ws.merge_count_cap * sizeof(int32_t));
-            return set_error(GKV_EDEVICE, "a kernel reported error bits 0x%x (1 = bad block id, 2 = wait timeout, 4 = bad slot, 8 = request left out of a built step)", flag);
+            return set_error(GKV_EDEVICE, "a kernel reported error bits 0x%x (1 = bad block id, 2 = wait timeout, 4 = bad slot, 8 = a request left out of a built step or a prompt out of its attention)", flag);
         }
     }
     return GKV_OK;

@@ -147,3 +147,15 @@ def test_batches_around_the_listing_limits(cuda, dtype, batch):
     lens = np.random.default_rng(batch).choice([0, 1, 3, 128, 130, 300], batch).tolist()
     q, k, v, cu = _inputs(lens, 2, 1, 64, 64, dtype, seed=batch)
     _check(q, k, v, cu, 0.125)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_a_left_out_prompt_is_named(cuda, dtype):
+    import torch
+
+    q, k, v, _ = _inputs([100], 2, 1, 64, 64, dtype, seed=25)
+    pool = G.PagedBlockPool(1, 1, 1, 64, 16)
+    pool.prompt_attention(q, k, v, torch.tensor([0, 101], dtype=torch.int32, device="cuda"), torch.empty_like(q), 0.125)
+    with pytest.raises(G.DeviceError, match="prompt"):
+        pool.sync()
+    pool.close()
