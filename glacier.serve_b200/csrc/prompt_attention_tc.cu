@@ -420,7 +420,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         // The blocks of the grid stand for the tiles, those with the most keys first (with a batch too large
         // to be listed, for each prompt), all heads of a tile in a row; some stand for none: the host knows
         // only total and batch.
-        if (blockIdx.x == 0) check_prompts(a, lane, 32);
         if (lane == 0) steal_block(bk->response, &bk->steal);  // the first answer is on its way meanwhile
         const int numbers = static_cast<int>(gridDim.x / a.n_heads);
         const int tiles = listed ? sum_prompt_levels(a, bk->list) : 0;
@@ -428,6 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t answers = 0;
         bool asking = true;
         while (true) {
+            if (block == 0) check_prompts(a, lane, 32);  // by whichever block has number 0, which may have been taken over too
             PromptTile pt;
             const int x = block / a.n_heads;
             bool found = false;
