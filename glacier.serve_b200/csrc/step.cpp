@@ -570,8 +570,19 @@ int step_build(Pool* p, const gkv_step_io* io, int32_t batch, cudaStream_t st) {
         return set_error(GKV_EINVAL, "ctx_lens/new_lens/block_tables is NULL");
     if (io->n_new_blocks > 0 && !io->d_new_blocks) return set_error(GKV_EINVAL, "new_blocks is NULL");
     if (batch > 0 && io->table_stride < 1) return set_error(GKV_EINVAL, "table_stride %d < 1", io->table_stride);
-    if (batch > 0 && (io->d_ctx_out == io->d_ctx_lens || io->d_ctx_out == io->d_new_lens))
-        return set_error(GKV_EINVAL, "ctx_out must not be ctx_lens or new_lens (every block of the kernel reads those)");
+    // every block of the kernel reads the inputs while others already write
+    const struct { const void* at; int64_t bytes; const char* name; } arrays[] = {
+        {io->d_ctx_lens, int64_t{4} * batch, "ctx_lens"}, {io->d_new_lens, int64_t{4} * batch, "new_lens"},
+        {io->d_new_blocks, int64_t{4} * io->n_new_blocks, "new_blocks"},
+        {io->d_block_tables, int64_t{4} * batch * io->table_stride, "block_tables"}, {io->d_ctx_out, int64_t{4} * batch, "ctx_out"},
+        {io->d_cu_new, int64_t{4} * (batch + 1), "cu_new"}, {io->d_slots, int64_t{8} * io->max_tokens, "slots"},
+        {io->d_positions, int64_t{4} * io->max_tokens, "positions"}, {io->d_counts, 8, "counts"}};
+    for (int o = 3; o < 9; ++o)
+        for (int i = 0; i < o; ++i) {
+            const uintptr_t x = reinterpret_cast<uintptr_t>(arrays[o].at), y = reinterpret_cast<uintptr_t>(arrays[i].at);
+            if (x && y && arrays[o].bytes > 0 && arrays[i].bytes > 0 && x < y + arrays[i].bytes && y < x + arrays[o].bytes)
+                return set_error(GKV_EINVAL, "%s overlaps %s", arrays[o].name, arrays[i].name);
+        }
     const int64_t workers = static_cast<int64_t>(ws.n_ctas_max) * ws.cfg.warps;
     const int64_t n_seg = static_cast<int64_t>(ws.max_batch) * p->desc.heads_kv;
     if (p->desc.heads_kv >= 1 << 10 || n_seg >= 1 << 20 || workers >= 1 << 14)

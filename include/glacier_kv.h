@@ -290,8 +290,8 @@ typedef struct gkv_step_io {
  * exceeds table_stride * block_size, its pages need more than n_new_blocks ids or its rows more
  * than max_tokens; all of them are left out of the decode (alone) when heads_kv times the chunks of 8
  * tokens they attend, plus 4 each, reach 2^31.  A block id outside the pool gives slot -1 and GKV_EDEVICE.  batch is at most
- * the reservation's and 4096, max_tokens at most the reservation's; d_ctx_out must not overlap
- * d_ctx_lens or d_new_lens.  No reference counterpart (the reference packs tables on the host,
+ * the reservation's and 4096, max_tokens at most the reservation's; the arrays that are written must
+ * overlap no other array of `io` (GKV_EINVAL).  No reference counterpart (the reference packs tables on the host,
  * CudaPagedTransformerRunner.cs:367-379). */
 GKV_API int gkv_step_build(gkv_pool* pool, const gkv_step_io* io, int32_t batch, void* stream);
 /* KV append (reshape-and-cache scatter) of the uploaded step's n_tok tokens:

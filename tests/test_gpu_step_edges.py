@@ -198,3 +198,40 @@ def test_prompts_and_tokens_in_one_step_then_a_further_chunk(cuda):
         ref, size, most = _attended(pool, rows[1], qn[i], have + i, scale)
         assert_within(chunk[i], ref, prompt_tolerance(ref, size, most, D, have + more, torch.float32)[0], f"chunk {i}")
     pool.close()
+
+
+def test_arrays_that_overlap_are_refused(cuda):
+    """A written array over any other, whole or by one element; arrays that only touch, and empty ones, are not over each other."""
+    import torch
+
+    pool = G.PagedBlockPool(8, 1, 2, 64, 16)
+    pool.reserve_step(4, 3, 6, 4)
+    pool.set_static_step()
+    # one buffer of int32 for all: place(name) gives each array's first element in it
+    sizes = {"d_ctx_lens": 4, "d_new_lens": 4, "d_new_blocks": 4, "d_block_tables": 12, "d_ctx_out": 4, "d_cu_new": 5, "d_slots": 12,
+             "d_positions": 6, "d_counts": 2}
+    buf = torch.zeros(64, dtype=torch.int32, device="cuda")
+    place, at = {}, 0
+    for name in ["d_slots"] + [n for n in sizes if n != "d_slots"]:  # 64-bit slots first: everything touches, nothing overlaps
+        place[name] = at
+        at += sizes[name]
+    io = G.StepBuffers(torch.zeros(4, 3, dtype=torch.int32, device="cuda"), _i32([0] * 4), _i32([0] * 4), _i32([0] * 4), max_tokens=6)
+
+    def build(**moved):
+        for name in sizes:
+            setattr(io._desc, name, buf.data_ptr() + 4 * {**place, **moved}[name])
+        pool.build_step(io)
+
+    build()
+    pool.sync()
+    order = sorted(place, key=place.get)
+    for before, name in zip(order, order[1:]):
+        if name in ("d_new_lens", "d_new_blocks") and before in ("d_ctx_lens", "d_new_lens"):
+            continue  # inputs may share memory
+        with pytest.raises(G.ArgumentOutOfRangeError, match="overlaps"):
+            build(**{name: place[name] - 1})
+    with pytest.raises(G.ArgumentOutOfRangeError, match="overlaps"):
+        build(d_cu_new=place["d_new_lens"])
+    build(d_new_lens=place["d_ctx_lens"])
+    pool.sync()
+    pool.close()
