@@ -3,9 +3,10 @@
 // gkv_rope_append's steps (bias, per-head RMSNorm of q and k, rotation, Store) for tokens whose
 // position has several axes, as image and video patches have: pair i of a head turns by
 //   angle_i = position[axis(i)] * inv_freq[i],   (a, b) -> (a cos - b sin, b cos + a sin) * mscale.
-// The angle is the exact product in 64 bits (31 + 24 bits of factors), reduced by pi/2 there and only
-// then rounded: at position 10^6 a product in 32 bits is off by up to 2^-5 rad.  Everything else is
-// 32 bits, rounded once to each destination's type.
+// The angle is formed in 64 bits: exact for positions below 2^29 (29 + 24 bits of factors), above off by
+// at most 2^-53 of itself, 2^-22 rad.  It is reduced by pi/2 there and only then rounded: at position
+// 10^6 a product in 32 bits is off by up to 2^-5 rad.  Everything else is 32 bits, rounded once to each
+// destination's type.
 //
 // Roofline: HBM for prompts, launch latency for single tokens.  A block takes up to 16 tokens (one
 // where there are few), puts their cos and sin into shared memory once for all heads, and hands

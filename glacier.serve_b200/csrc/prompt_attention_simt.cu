@@ -12,7 +12,8 @@
 // while they are used.
 //
 // Measured (32 q and 8 kv heads of 128, 32 bits): 4 prompts of 4096 tokens 45 TFLOP/s, 60 % of the FMA rate of
-// 74.5; 6 ragged prompts of 1 to 1500 tokens 0.70 ms = 36.5 TFLOP/s.  A key tile takes 13.5 us where its FMAs take
+// 74.5; 6 ragged prompts of 1 to 1500 tokens 0.71 ms = 36.4 TFLOP/s; bf16 with head dims of 96, 256 and 192/128, which
+// the tensor-core kernel does not take, 30 to 37 TFLOP/s.  A key tile takes 13.5 us where its FMAs take
 // 8.3: shared memory gives 128 bytes a cycle to the registers, which the values (4 FMA a float) just live on
 // and the scores (8 / 3 FMA a float) do not, and one block of 8 warps an SM (184 KB) hides little of the softmax.
 #include "gkv_device.cuh"

@@ -31,12 +31,14 @@
 // Every wait is bounded: on expiry the block raises kErrWaitTimeout, lets its copies and products
 // finish, frees its tensor memory and ends.
 //
-// Measured (28 q and 4 kv heads of 128, bf16): 16384 tokens 1.38 ms = 1394 TFLOP/s, 83 % of the measured
-// product rate, and 1.6 ms where the card holds its power limit; tensor pipe and exponentials are each busy for
-// 71 % of the time.  24 prompts of 1 to 6000 tokens: 0.53 ms = 1100 TFLOP/s, first and last key tiles.  16 q
-// and 4 kv heads of 64 in fp16, 9 prompts of up to 4000 tokens: 0.137 ms = 590 TFLOP/s; with half the
-// products for the same exponentials those are the bound (0.068 ms), and short items leave the chain of
-// scores, softmax and P V bare.
+// Measured (28 q and 4 kv heads of 128, bf16), with the SM clock sampled meanwhile: 16384 tokens 1.38 ms = 1394
+// TFLOP/s at 1965 MHz, 83 % of the measured product rate, and 1.60 ms = 1200 TFLOP/s at the 1550 MHz that the
+// power limit leaves after some 0.3 s back to back; tensor pipe and exponentials are each busy for 71 % of the time.  24
+// prompts of 1 to 6000 tokens: 0.527 ms = 1107 TFLOP/s at 1965 MHz, 0.616 ms = 948 at the power limit's
+// 1597, and some 0.63 ms for a first call whose inputs are in no cache; first and last key tiles.  16 q and 4 kv
+// heads of 64 in fp16, 9 prompts of up to 4000 tokens: 0.136 ms = 594 TFLOP/s at 1965 MHz, 0.17 ms with cold caches; with
+// half the products for the same exponentials those are the bound (0.068 ms), and short items leave the
+// chain of scores, softmax and P V bare.
 #include <cuda.h>
 
 #include <atomic>

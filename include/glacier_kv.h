@@ -414,7 +414,8 @@ typedef struct gkv_prompt_desc {
  * runs in both step layouts and in a captured graph, and offers sinks and lse.  heads_kv, head_dim
  * and v_head_dim are the pool's; the arena's type does not matter.  16-bit types with head_dim =
  * v_head_dim = 64 or 128 and scale > 0 run on the tensor cores (p rounded to the inputs' type
- * before p . v), the others in 32-bit arithmetic; softmax statistics are 32 bits.  Masked keys and
+ * before p . v), the others, and strides that a tensor map does not hold (2^40 bytes and more),
+ * in 32-bit arithmetic, which takes 25 to 30 times as long; softmax statistics are 32 bits.  Masked keys and
  * values, and rows of other requests, never reach a result, whatever they hold.  Rows behind
  * cu_seqlens[batch] are left alone.  A prompt whose range is negative or passes `total` is left out
  * (GKV_EDEVICE from the next gkv_sync); the others keep their results where their rows follow one
