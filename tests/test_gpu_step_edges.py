@@ -235,3 +235,37 @@ def test_arrays_that_overlap_are_refused(cuda):
     build(d_new_lens=place["d_ctx_lens"])
     pool.sync()
     pool.close()
+
+
+@pytest.mark.parametrize("dtype,heads,heads_kv,dim", [("f32", 4, 2, 64), ("bf16", 28, 4, 128), ("fp8", 28, 4, 128)])
+def test_decode_over_a_table_with_a_bad_id(cuda, dtype, heads, heads_kv, dim):
+    """The build takes earlier table entries as they are: an id outside the pool is reported, and the other requests are served."""
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(34)
+    B, width = 3, 8
+    pool = G.PagedBlockPool(B * width, 1, heads_kv, dim, 16, dtype=dtype)
+    for view in (pool.key_view(), pool.value_view()):
+        x = torch.randn(view.shape, device="cuda", generator=g)
+        view.copy_(x.to(torch.float8_e4m3fn).view(torch.uint8) if dtype == "fp8" else x)
+    pool.reserve_step(B, width, B, heads)
+    pool.set_static_step()
+    tables = torch.arange(B * width, dtype=torch.int32, device="cuda").view(B, width)
+    q = torch.randn(B, heads, dim, device="cuda", generator=g)
+    outs = []
+    for bad in (None, B * width, -1, 2 ** 31 - 1, None):
+        t = tables.clone()
+        if bad is not None:
+            t[1, 3] = bad
+        out = torch.full((B, heads, dim), 7.0, device="cuda")
+        pool.build_step(G.StepBuffers(t, _i32([100, 128, 17]), _i32([0] * B), _i32([]), max_tokens=B))
+        pool.paged_decode(0, q, out, heads, 1 / math.sqrt(dim))
+        if bad is not None:
+            with pytest.raises(G.DeviceError):
+                pool.sync()
+        pool.sync()
+        outs.append(out)
+    assert torch.equal(outs[0], outs[-1]) and bool(outs[0].isfinite().all())
+    for out in outs[1:-1]:
+        assert torch.equal(out[[0, 2]], outs[0][[0, 2]])
+    pool.close()
